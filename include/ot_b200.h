@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define OT_B200_ABI_VERSION 3
+#define OT_B200_ABI_VERSION 4
 
 typedef enum ot_b200_status {
   OT_B200_OK = 0,
@@ -296,6 +296,51 @@ int ot_b200_backward_linear(const void *d_x, const void *d_w, const float *d_bia
                             int64_t rows, int32_t D, int32_t V, int32_t max_u, int32_t blank,
                             uint32_t flags, const void *d_workspace, uint64_t workspace_bytes,
                             void *d_grad_logits, const float *d_scale, double scale_host, void *stream);
+
+/* ---- The output projection in 8-bit floating point --------------------------
+ * out[m, n] = sum_kb sa[kb][m] * sb[n / 128][kb] * (sum_{k in kb} a[m,k] b[n,k]) (+ bias[n])
+ * with a (M, K) and b (N, K) in e4m3 and one float scale for every block of 128
+ * elements along K: 1 x 128 for a, 128 x 128 for b (the last block of either axis may
+ * be shorter).  The products of a block are summed by the tensor cores in float, the
+ * blocks' sums scaled and added in float registers, and the result is rounded once.
+ * No counterpart in the reference, which is given the logits.
+ *
+ * ot_b200_fp8_quantize writes x (rows, cols; unit column stride, rows row_stride
+ * elements apart; float, or as OT_B200_BF16 / OT_B200_FP16 in `flags` says) in e4m3, from
+ * one read of x, with the scale of a block the smallest power of two s for which
+ * max|x| <= 448 s (2^-126 at least; 1 for a block of zeros; NaN for a block that holds an
+ * infinity or a NaN):
+ *   d_q      (rows, cols) bytes, rows q_pitch bytes apart (a multiple of 16; base 16-byte aligned)
+ *   d_scale  blocks of 1 x 128: [ceil(cols/128)][rows];  128 x 128: [ceil(rows/128)][ceil(cols/128)]
+ *   d_qt     (cols, rows) bytes, rows qt_pitch = rows rounded up to 16 bytes apart, or NULL
+ *   d_scale_t  blocks of 128 x 1 (of x): [ceil(rows/128)][cols];  128 x 128: [ceil(cols/128)][ceil(rows/128)]
+ *   d_column_sums  (cols) float sums of x over its rows, or NULL; then d_partial_sums holds
+ *            ceil(rows/128) * cols floats of scratch (mode ..._ROWS_AND_COLUMNS only)
+ * so (d_q, d_scale) in blocks of 1 x 128 is an `a`, in blocks of 128 x 128 a `b`, and the
+ * transposed pair the same for x^T. */
+typedef enum ot_b200_fp8_mode {
+  OT_B200_FP8_ROWS = 0,              /* q in 1 x 128                                       */
+  OT_B200_FP8_SQUARES = 1,           /* q in 128 x 128                                     */
+  OT_B200_FP8_ROWS_AND_SQUARES = 2,  /* q in 1 x 128, q^T in 128 x 128                     */
+  OT_B200_FP8_SQUARES_BOTH = 3,      /* q and q^T in 128 x 128                             */
+  OT_B200_FP8_ROWS_AND_COLUMNS = 4   /* q in 1 x 128, q^T in 1 x 128 of x^T                */
+} ot_b200_fp8_mode;
+int ot_b200_fp8_quantize(const void *d_x, int64_t rows, int32_t cols, int64_t row_stride, uint32_t flags,
+                         int32_t mode, void *d_q, int64_t q_pitch, float *d_scale, void *d_qt,
+                         int64_t qt_pitch, float *d_scale_t, float *d_partial_sums,
+                         float *d_column_sums, void *stream);
+
+/* The product.  d_out (M, N) contiguous, float or as OT_B200_BF16 / OT_B200_FP16 say;
+ * d_a, d_b 16-byte aligned, their pitches (bytes from row to row) multiples of 16;
+ * d_bias (N) float or NULL.  When K is long and M x N small the work is split along K
+ * and the pieces' sums are joined in a fixed order: the workspace (16-byte aligned) holds
+ * them, 0 bytes otherwise.  `flags` may hold OT_B200_REPORT_ERRORS: a wait of the kernel
+ * that ran out (never in normal operation) is then recorded for the next call. */
+int ot_b200_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, uint64_t *bytes_out);
+int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a, const void *d_b,
+                       int64_t b_pitch, const float *d_scale_b, const float *d_bias, int64_t M,
+                       int64_t N, int64_t K, uint32_t flags, void *d_workspace,
+                       uint64_t workspace_bytes, void *d_out, void *stream);
 
 /* d_grad[i] *= *d_scale for i < count, unless *d_scale == 1 (then the buffer is
  * not touched: the kernel's blocks return after one load).  The counterpart of

@@ -9,7 +9,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libot_b200.so")
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 # ot_b200_status
 OK, ERR_ARGUMENT, ERR_CUDA, ERR_WORKSPACE, ERR_INPUT = range(5)
@@ -28,6 +28,9 @@ TRACE = 512
 REPORT_ERRORS = 1024
 LINEAR_DOMAIN = 2048
 
+# ot_b200_fp8_mode
+(FP8_ROWS, FP8_SQUARES, FP8_ROWS_AND_SQUARES, FP8_SQUARES_BOTH, FP8_ROWS_AND_COLUMNS) = range(5)
+
 # Every symbol include/ot_b200.h declares.
 EXPORTS = (
     "ot_b200_abi_version",
@@ -41,6 +44,9 @@ EXPORTS = (
     "ot_b200_scale_gradient",
     "ot_b200_forward_linear",
     "ot_b200_backward_linear",
+    "ot_b200_fp8_quantize",
+    "ot_b200_fp8_matmul_workspace_bytes",
+    "ot_b200_fp8_matmul",
     "ot_b200_compute_transducer_loss",
     "ot_b200_poll_errors",
     "ot_b200_read_input_status",
@@ -106,6 +112,12 @@ def load():
     lib.ot_b200_backward_linear.restype = ctypes.c_int
     lib.ot_b200_backward_linear.argtypes = [vp, vp, vp, i32, i64, i32, i32, i32, i32, u32, vp, u64, vp, vp,
                                             ctypes.c_double, vp]
+    lib.ot_b200_fp8_quantize.restype = ctypes.c_int
+    lib.ot_b200_fp8_quantize.argtypes = [vp, i64, i32, i64, u32, i32, vp, i64, vp, vp, i64, vp, vp, vp, vp]
+    lib.ot_b200_fp8_matmul_workspace_bytes.restype = ctypes.c_int
+    lib.ot_b200_fp8_matmul_workspace_bytes.argtypes = [i64, i64, i64, ctypes.POINTER(u64)]
+    lib.ot_b200_fp8_matmul.restype = ctypes.c_int
+    lib.ot_b200_fp8_matmul.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, u32, vp, u64, vp, vp]
     lib.ot_b200_scale_gradient.restype = ctypes.c_int
     lib.ot_b200_scale_gradient.argtypes = [vp, i64, vp, u32, vp]
     lib.ot_b200_compute_transducer_loss.restype = ctypes.c_int

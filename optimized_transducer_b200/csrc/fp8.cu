@@ -1,0 +1,741 @@
+// The joiner's output projection in 8-bit floating point (e4m3) with one float scale
+// for every block of 128 elements along the contraction:
+//
+//   out[m, n] = sum_kb sa[m, kb] * sb[n / 128, kb] * ( sum_{k in block kb} a[m, k] * b[n, k] )  (+ bias[n])
+//
+// a (M, K) has blocks of 1 x 128, b (N, K) blocks of 128 x 128.  Three products of a
+// training step have this form, each with both operands stored along the contraction:
+//   logits = x * W^T       a = x (rows, D)         b = W (V, D)
+//   dX     = dY * W        a = dY (rows, V)        b = W^T (D, V)
+//   dW     = dY^T * X      a = dY^T (V, rows)      b = X^T (D, rows)
+// so the quantiser below writes a tile plain, transposed, or both from one read.  The
+// reference has no counterpart: it takes the logits as they are
+// (optimized_transducer/csrc/transducer-loss.h:60-63).
+//
+// Scales.  quantize_kernel takes the smallest power of two s with max|x| / s <= 448 (the
+// largest e4m3 value), 2^-126 at least, 1 for a block of zeros: x / s is then exact but
+// for the rounding to e4m3 itself, and since e4m3 is a floating-point type a scale that is
+// not a power of two would not round less.  A block that holds an infinity or a NaN gets
+// the scale NaN: every product with it is NaN, as it would be without the quantiser.  The
+// product takes any float scales (a checkpoint's).
+#include <cuda_fp8.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "ot_common.cuh"
+#include "tensor_core.cuh"
+
+namespace otb {
+
+namespace {
+
+constexpr int kScaleBlock = 128;  // elements of the contraction that share a scale
+constexpr int kQuantThreads = 256;
+constexpr int kQuantRows = kScaleBlock / (kQuantThreads / 32);  // rows of a tile per warp
+
+int fail(int code, const char *fmt, ...) {
+  char msg[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  set_last_error(msg);
+  return code;
+}
+
+// ---------------------------------------------------------------------------
+// quantisation
+// ---------------------------------------------------------------------------
+// Scale of a block whose largest magnitude has the float bits `top` (bits of |x| order as
+// unsigned integers do, NaN above infinity), and its reciprocal; both exact.
+__device__ __forceinline__ float block_scale(uint32_t top, float &inverse) {
+  if (top == 0u) { inverse = 1.f; return 1.f; }
+  if (top >= 0x7f800000u) { inverse = __int_as_float(0x7fffffff); return inverse; }
+  // |x| = f * 2^(e - 127) with 1 <= f < 2; 448 = 1.75 * 2^8
+  int k = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  k = k < -126 ? -126 : k;
+  inverse = __int_as_float((127 - k) << 23);
+  return __int_as_float((127 + k) << 23);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+template <typename T> __device__ __forceinline__ float to_float(T x) { return (float)x; }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]);
+template <> __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
+  const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]) {
+  const uint2 a = __ldg(reinterpret_cast<const uint2 *>(p));
+  T t[4];
+  memcpy(t, &a, sizeof(a));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = to_float(t[i]);
+}
+
+enum { kNone = 0, kRowBlocks = 1, kSquareBlocks = 2, kColumnBlocks = 1 };
+
+struct QuantArgs {
+  int64_t rows, ld;     // ld: elements from one row of x to the next
+  int cols, col_tiles;
+  bool vec;             // every group of four columns may be loaded at once
+  uint8_t *q;           // (rows, cols), rows q_pitch bytes apart
+  int64_t q_pitch;
+  float *scale;         // kRowBlocks: [column tile][row]; kSquareBlocks: [row tile][column tile]
+  uint8_t *qt;          // (cols, rows), rows qt_pitch bytes apart
+  int64_t qt_pitch;
+  float *scale_t;       // kColumnBlocks: [row tile][column]; kSquareBlocks: [column tile][row tile]
+  int64_t row_tiles;
+  float *column_sums;   // [row tile][column], or NULL
+};
+
+// One block per 128 x 128 tile of x; a warp holds 16 rows, a lane four columns of each, in
+// registers, so the tile is read once whatever is written: bytes along the rows (kPlain),
+// transposed bytes (kTrans), and the tile's column sums.  Bound by HBM: sizeof(T) bytes
+// read and one or two written per element.
+template <typename T, int kPlain, int kTrans, bool kSums>
+__global__ void __launch_bounds__(kQuantThreads)
+quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
+  __shared__ uint32_t top_s[8][kScaleBlock];   // column maxima of each warp (or one word per warp)
+  __shared__ float sum_s[kSums ? 8 : 1][kScaleBlock];
+  __shared__ float inv_s[kScaleBlock];
+  __shared__ __align__(16) uint8_t tile_s[kTrans != kNone ? kScaleBlock * kScaleBlock : 16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rt = blockIdx.x / a.col_tiles;
+  const int ct = (int)(blockIdx.x - rt * a.col_tiles);
+  const int64_t row0 = rt * kScaleBlock + warp * kQuantRows;
+  const int col0 = ct * kScaleBlock, col = col0 + 4 * lane;
+  pdl_wait();
+  pdl_trigger();
+
+  float v[kQuantRows][4];
+#pragma unroll
+  for (int i = 0; i < kQuantRows; ++i) {
+    const int64_t row = row0 + i;
+    const T *p = x + row * a.ld + col;
+    v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+    if (row < a.rows) {
+      if (a.vec && col + 3 < a.cols) {
+        load4<T>(p, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < a.cols) v[i][j] = to_float(p[j]);
+      }
+    }
+  }
+
+  if constexpr (kPlain == kRowBlocks) {
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < kQuantRows; ++i) {
+      uint32_t top = max(max(abs_bits(v[i][0]), abs_bits(v[i][1])), max(abs_bits(v[i][2]), abs_bits(v[i][3])));
+      top = __reduce_max_sync(kFull, top);
+      float inv;
+      const float s = block_scale(top, inv);
+      if (lane == i) mine = s;
+      if (row0 + i < a.rows && col < a.cols)  // the pitch is a multiple of 16: the word stays inside the row
+        *reinterpret_cast<uint32_t *>(a.q + (row0 + i) * a.q_pitch + col) =
+            pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+    }
+    if (lane < kQuantRows && row0 + lane < a.rows) a.scale[(int64_t)ct * a.rows + row0 + lane] = mine;
+  }
+  float square_inv = 0.f;
+  if constexpr (kPlain == kSquareBlocks || kTrans == kSquareBlocks) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < kQuantRows; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, abs_bits(v[i][j]));
+    top = __reduce_max_sync(kFull, top);
+    if (lane == 0) top_s[0][warp] = top;
+    __syncthreads();
+    top = 0u;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = max(top, top_s[0][w]);
+    const float s = block_scale(top, square_inv);
+    if (threadIdx.x == 0) {
+      if (kPlain == kSquareBlocks) a.scale[rt * a.col_tiles + ct] = s;
+      if (kTrans == kSquareBlocks) a.scale_t[(int64_t)ct * a.row_tiles + rt] = s;
+    }
+    if (kPlain == kSquareBlocks) {
+#pragma unroll
+      for (int i = 0; i < kQuantRows; ++i)
+        if (row0 + i < a.rows && col < a.cols)
+          *reinterpret_cast<uint32_t *>(a.q + (row0 + i) * a.q_pitch + col) =
+              pack4(v[i][0] * square_inv, v[i][1] * square_inv, v[i][2] * square_inv, v[i][3] * square_inv);
+    }
+  }
+  if constexpr (kTrans == kColumnBlocks || kSums) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t top = 0u;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kQuantRows; ++i) {
+        top = max(top, abs_bits(v[i][j]));
+        sum += v[i][j];
+      }
+      if (kTrans == kColumnBlocks) top_s[warp][4 * lane + j] = top;
+      if (kSums) sum_s[warp][4 * lane + j] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < kScaleBlock) {
+      const int c = threadIdx.x;
+      if (kTrans == kColumnBlocks) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) top = max(top, top_s[w][c]);
+        float inv;
+        const float s = block_scale(top, inv);
+        inv_s[c] = inv;
+        if (col0 + c < a.cols) a.scale_t[rt * a.cols + col0 + c] = s;
+      }
+      if (kSums) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += sum_s[w][c];
+        if (col0 + c < a.cols) a.column_sums[rt * a.cols + col0 + c] = sum;
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (kTrans != kNone) {
+    // A lane's 16 rows of one column are 16 consecutive bytes of the transposed tile.  The
+    // 16-byte pieces of a column are permuted by the column's group of four, so that the
+    // eight lanes of a store phase (columns four apart) hit different banks.
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float inv = kTrans == kSquareBlocks ? square_inv : inv_s[4 * lane + j];
+      uint4 w;
+      w.x = pack4(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
+      w.y = pack4(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv);
+      w.z = pack4(v[8][j] * inv, v[9][j] * inv, v[10][j] * inv, v[11][j] * inv);
+      w.w = pack4(v[12][j] * inv, v[13][j] * inv, v[14][j] * inv, v[15][j] * inv);
+      *reinterpret_cast<uint4 *>(tile_s + (4 * lane + j) * kScaleBlock + 16 * (warp ^ (lane & 7))) = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = threadIdx.x; i < kScaleBlock * 8; i += kQuantThreads) {
+      const int c = i >> 3, piece = i & 7;
+      const int64_t at = rt * kScaleBlock + 16 * piece;
+      if (col0 + c < a.cols && at < a.qt_pitch)
+        *reinterpret_cast<uint4 *>(a.qt + (int64_t)(col0 + c) * a.qt_pitch + at) =
+            *reinterpret_cast<const uint4 *>(tile_s + c * kScaleBlock + 16 * (piece ^ ((c >> 2) & 7)));
+    }
+  }
+}
+
+// Column sums from the tiles' partial sums, in a fixed order: a block adds the partials of
+// 8 columns with 32 threads each, then the 32 sums by a tree.
+__global__ void __launch_bounds__(256)
+column_sum_kernel(const float *__restrict__ part, int64_t row_tiles, int cols, float *__restrict__ out) {
+  __shared__ float s[32][9];
+  pdl_wait();
+  pdl_trigger();
+  const int c = threadIdx.x & 7, g = threadIdx.x >> 3;
+  const int col = blockIdx.x * 8 + c;
+  float sum = 0.f;
+  if (col < cols)
+    for (int64_t r = g; r < row_tiles; r += 32) sum += __ldg(part + r * cols + col);
+  s[g][c] = sum;
+  __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) {
+    if (g < o) s[g][c] += s[g + o][c];
+    __syncthreads();
+  }
+  if (g == 0 && col < cols) out[col] = s[0][c];
+}
+
+// ---------------------------------------------------------------------------
+// the product
+// ---------------------------------------------------------------------------
+constexpr int kTileM = 128;                      // rows per tile = TMEM lanes
+constexpr int kMmaK = 32;                        // K of one tcgen05.mma for 8-bit operands
+constexpr uint32_t kBytesA = kTileM * kScaleBlock;
+constexpr int kStagePitch = 80;                  // bytes from row to row of a warp's 32 x 64-byte staging tile
+
+// Columns per tile: 256, 128 or 64.  Every epilogue warp owns 32 rows x 64 columns.
+template <int kTileN> struct Shape {
+  static constexpr int epilogue_warps = kTileN / 16;
+  static constexpr int threads = 64 + 32 * epilogue_warps;
+  static constexpr uint32_t stage_bytes = kBytesA + kTileN * kScaleBlock;
+  static constexpr int ring = kTileN == 256 ? 3 : (kTileN == 128 ? 5 : 6);
+  static constexpr int accumulators = kTileN == 256 ? 2 : 4;
+  static constexpr uint32_t tmem_columns = accumulators * kTileN;
+  static constexpr size_t smem = 1024 + (size_t)ring * stage_bytes + (size_t)epilogue_warps * 32 * kStagePitch;
+  // kind::f8f6f4: float accumulator (bits [4,6) = 1), e4m3 A and B (0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+  static constexpr uint32_t instr = (1u << 4) | ((uint32_t)(kTileN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+};
+
+__device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t instr, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(instr), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_load_16_issue(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load_16_wait(uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+      :
+      : "memory");
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);  // 16-bit types
+template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) { return Pair16<__nv_bfloat16>::round(a, b); }
+template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) { return Pair16<__half>::round(a, b); }
+
+// Copies a staged 32-row x 64-byte tile to rows of out that are `pitch` bytes apart, in
+// units of sizeof(U) bytes: a store instruction covers whole pieces of rows.
+template <typename U>
+__device__ __forceinline__ void store_staged(const unsigned char *staged, unsigned char *out, int64_t pitch, int rows, int bytes, int lane) {
+  constexpr int kUnits = 64 / sizeof(U);                 // units per row
+  constexpr int kRows = kUnits >= 32 ? 1 : 32 / kUnits;  // rows per instruction
+  const int unit = lane % kUnits, r0 = lane / kUnits;
+  if (unit * (int)sizeof(U) >= bytes) return;
+#pragma unroll 4
+  for (int r = r0; r < rows; r += kRows)
+    *reinterpret_cast<U *>(out + r * pitch + unit * sizeof(U)) =
+        *reinterpret_cast<const U *>(staged + r * kStagePitch + unit * sizeof(U));
+}
+
+struct MatmulArgs {
+  const float *sa;      // [K block][M]
+  const float *sb;      // [N / 128][K block]
+  const float *bias;    // [N] or NULL
+  unsigned char *out;   // (splits, M, N): splits > 1 holds partial sums
+  int64_t M;
+  int N, k_blocks, n_tiles, splits;
+  int64_t tiles;
+  int unit;             // bytes per store: the largest of 16, 8, 4, 2 that divides the rows' pitch and the base
+  int32_t *sticky;      // error record, or NULL
+  int32_t seq;
+};
+
+template <int kTileN> struct MatmulShared {
+  uint64_t full[Shape<kTileN>::ring];          // TMA -> MMA
+  uint64_t empty[Shape<kTileN>::ring];         // MMA -> TMA
+  uint64_t acc_full[Shape<kTileN>::accumulators];   // MMA -> epilogue: one K block's product is complete
+  uint64_t acc_empty[Shape<kTileN>::accumulators];  // epilogue -> MMA
+  uint32_t tmem_base;
+  int never;
+  volatile int abort;
+  alignas(16) float bias[Shape<kTileN>::epilogue_warps][64];  // read as float4
+};
+
+// One CTA per SM, persistent over (row tile, column tile, piece of K).  The scales change
+// with every K block, so a block's product is complete in tensor memory on its own (four
+// MMAs of K = 32) and the epilogue adds it, scaled, to sums held in registers in float:
+// one multiply-add per element and K block, which runs while the tensor cores work on the
+// next block's product.  Per K block the MMAs take kTileN * 2 cycles; the sixteen epilogue
+// warps of the widest tile need 64 multiply-adds and four 16-column reads each.
+//   warp 0   TMA producer: a (128 x 128) and b (kTileN x 128) boxes into the ring
+//   warp 1   MMA issuer
+//   others   epilogue: warp % 4 picks the TMEM lanes (rows), the rest the 64 columns
+// A wait that runs out raises the CTA's abort flag; every role leaves, the producer waits
+// (bounded) for its copies in flight, and the record of the failure goes to `sticky`.
+template <int kTileN, typename OutT>
+__global__ void __launch_bounds__(Shape<kTileN>::threads, 1)
+fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulArgs g) {
+  using S = Shape<kTileN>;
+  constexpr int R = S::ring, B = S::accumulators;
+  extern __shared__ __align__(1024) unsigned char ring_mem[];
+  __shared__ MatmulShared<kTileN> sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char *ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(ring_mem) + 1023) & ~uintptr_t(1023));
+  unsigned char *staging = ring + (size_t)R * S::stage_bytes;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < R; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+    for (int i = 0; i < B; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], 32 * S::epilogue_warps); }
+    sh.abort = 0;
+    sh.never = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  pdl_wait();  // before the allocation: a predecessor's blocks may still hold tensor memory
+  pdl_trigger();
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&sh.tmem_base)), "r"(S::tmem_columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sh.tmem_base;
+
+  // tile -> (piece of K, row tile, column tile), the column tile fastest: the row tile's
+  // bytes are read once from HBM and again from L2
+  const auto place = [&](int64_t tile, int &nt, int64_t &mt, int &sp, int &k0, int &k1) {
+    nt = (int)(tile % g.n_tiles);
+    const int64_t rest = tile / g.n_tiles;
+    sp = (int)(rest % g.splits);
+    mt = rest / g.splits;
+    k0 = (int)((int64_t)g.k_blocks * sp / g.splits);
+    k1 = (int)((int64_t)g.k_blocks * (sp + 1) / g.splits);
+  };
+
+  if (warp == 0 && lane == 0) {
+    uint32_t it = 0;
+    for (int64_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
+      int nt, sp, k0, k1;
+      int64_t mt;
+      place(tile, nt, mt, sp, k0, k1);
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % R;
+        if (it >= R && !mbar_wait(&sh.empty[s], ((it / R) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+        unsigned char *a = ring + (size_t)s * S::stage_bytes;
+        mbar_expect_tx(&sh.full[s], S::stage_bytes);
+        // what lies beyond either matrix is filled with zeros by the copy
+        tma_load_2d(a, &map_a, kb * kScaleBlock, (int)(mt * kTileM), &sh.full[s]);
+        tma_load_2d(a + kBytesA, &map_b, kb * kScaleBlock, nt * kTileN, &sh.full[s]);
+      }
+    }
+    if (sh.abort) {
+      const volatile int *never = &sh.never;
+      for (uint32_t j = (it > R ? it - R : 0); j < it; ++j) mbar_wait(&sh.full[j % R], (j / R) & 1, never);
+      if (g.sticky != nullptr) {
+        volatile int32_t *r = g.sticky;
+        r[1] = 0;
+        r[2] = g.seq;
+        __threadfence_system();
+        r[0] = OT_B200_COPY_TIMEOUT;
+      }
+    }
+  } else if (warp == 1 && lane == 0) {
+    uint32_t it = 0;
+    for (int64_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
+      int nt, sp, k0, k1;
+      int64_t mt;
+      place(tile, nt, mt, sp, k0, k1);
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % R, buf = it % B;
+        if (it >= B && !mbar_wait(&sh.acc_empty[buf], ((it / B) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+        if (!mbar_wait(&sh.full[s], (it / R) & 1, &sh.abort)) { sh.abort = 1; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t a = smem_u32(ring + (size_t)s * S::stage_bytes);
+        const uint64_t da = smem_desc(a), db = smem_desc(a + kBytesA);
+#pragma unroll
+        for (int k = 0; k < kScaleBlock / kMmaK; ++k)  // 32 bytes further along K inside the swizzle row
+          mma_f8(tmem + (uint32_t)(buf * kTileN), da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), S::instr, k != 0);
+        mma_commit(&sh.empty[s]);
+        mma_commit(&sh.acc_full[buf]);
+      }
+    }
+  } else if (warp >= 2) {
+    const int quarter = warp & 3;
+    const int part = (warp - 2) >> 2;
+    unsigned char *staged = staging + (size_t)(warp - 2) * 32 * kStagePitch;
+    uint32_t it = 0;
+    bool dead = false;  // the same for all lanes: the reads of tensor memory are warp-wide
+    for (int64_t tile = blockIdx.x; tile < g.tiles && !dead; tile += gridDim.x) {
+      int nt, sp, k0, k1;
+      int64_t mt;
+      place(tile, nt, mt, sp, k0, k1);
+      const int64_t row0 = mt * kTileM + quarter * 32;
+      const int64_t row = row0 + lane;
+      const int col0 = nt * kTileN + part * 64;
+      const bool live = row < g.M;
+      const float *sa = g.sa + (live ? row : 0);
+      const float *sb = g.sb + (int64_t)min(col0 / kScaleBlock, (g.N - 1) / kScaleBlock) * g.k_blocks;
+      __syncwarp();  // the previous tile's bias has been read
+      sh.bias[warp - 2][lane] = (g.bias != nullptr && col0 + lane < g.N) ? __ldg(g.bias + col0 + lane) : 0.f;
+      sh.bias[warp - 2][lane + 32] = (g.bias != nullptr && col0 + 32 + lane < g.N) ? __ldg(g.bias + col0 + 32 + lane) : 0.f;
+      float acc[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i] = 0.f;
+      float s_next = k0 < k1 ? __ldg(sa + (int64_t)k0 * g.M) * __ldg(sb + k0) : 0.f;
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int buf = it % B;
+        const float s = s_next;
+        if (kb + 1 < k1) s_next = __ldg(sa + (int64_t)(kb + 1) * g.M) * __ldg(sb + kb + 1);
+        dead = !__all_sync(kFull, mbar_wait(&sh.acc_full[buf], (it / B) & 1, &sh.abort));
+        if (dead) { sh.abort = 1; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kTileN + part * 64);
+        uint32_t r[2][16];
+        tmem_load_16_issue(taddr, r[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_load_16_wait(r[c & 1]);
+          if (c < 3) {
+            tmem_load_16_issue(taddr + 16 * (c + 1), r[(c + 1) & 1]);
+          } else {  // the last read has landed: the accumulator goes back
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(&sh.acc_empty[buf]);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(s, __uint_as_float(r[c & 1][i]), acc[16 * c + i]);
+        }
+      }
+      if (dead) break;
+      __syncwarp();
+      {
+        const float4 *b = reinterpret_cast<const float4 *>(sh.bias[warp - 2]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float4 v = b[i];
+          acc[4 * i] += v.x; acc[4 * i + 1] += v.y; acc[4 * i + 2] += v.z; acc[4 * i + 3] += v.w;
+        }
+      }
+      // rows leave through the warp's staging tile, 64 bytes of each at a time
+      constexpr int kChunk = 64 / (int)sizeof(OutT);
+      const int rows_here = (int)min((int64_t)32, g.M - row0);
+      unsigned char *out = g.out + ((int64_t)sp * g.M + row0) * g.N * (int64_t)sizeof(OutT) + (int64_t)col0 * sizeof(OutT);
+      const int64_t pitch = (int64_t)g.N * sizeof(OutT);
+#pragma unroll
+      for (int c = 0; c < 64 / kChunk; ++c) {
+        const int bytes = min(64, (g.N - col0) * (int)sizeof(OutT) - c * 64);
+        if (bytes <= 0 || rows_here <= 0) break;  // warp-uniform
+        uint4 *mine = reinterpret_cast<uint4 *>(staged + lane * kStagePitch);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint4 w;
+          if constexpr (sizeof(OutT) == 4) {
+            w = make_uint4(__float_as_uint(acc[16 * c + 4 * i]), __float_as_uint(acc[16 * c + 4 * i + 1]),
+                           __float_as_uint(acc[16 * c + 4 * i + 2]), __float_as_uint(acc[16 * c + 4 * i + 3]));
+          } else {
+            const float *p = acc + 32 * c + 8 * i;
+            w = make_uint4(pack_pair<OutT>(p[0], p[1]), pack_pair<OutT>(p[2], p[3]), pack_pair<OutT>(p[4], p[5]), pack_pair<OutT>(p[6], p[7]));
+          }
+          mine[i] = w;
+        }
+        __syncwarp();
+        if (g.unit == 16) store_staged<uint4>(staged, out + c * 64, pitch, rows_here, bytes, lane);
+        else if (g.unit == 8) store_staged<uint2>(staged, out + c * 64, pitch, rows_here, bytes, lane);
+        else if (g.unit == 4) store_staged<uint32_t>(staged, out + c * 64, pitch, rows_here, bytes, lane);
+        else store_staged<uint16_t>(staged, out + c * 64, pitch, rows_here, bytes, lane);
+        __syncwarp();
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::tmem_columns) : "memory");
+}
+
+// out = sum over the pieces of K (in their order) + bias, rounded once.
+template <typename OutT>
+__global__ void __launch_bounds__(256)
+split_sum_kernel(const float *__restrict__ part, int splits, int64_t count, int N, const float *__restrict__ bias, OutT *__restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    float sum = bias != nullptr ? __ldg(bias + i % N) : 0.f;
+    for (int s = 0; s < splits; ++s) sum += __ldg(part + (int64_t)s * count + i);
+    out[i] = (OutT)sum;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+struct MatmulPlan { int tile_n, splits; };
+
+// Columns per tile: the widest tile that still gives every SM a tile of its own (per K
+// block a wide tile reads fewer bytes of shared memory per product); a narrower N wants no
+// wider tile.  Pieces of K: only when even then most SMs would idle and K is long (dW: K is
+// the number of rows), at least eight blocks of K each.
+MatmulPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
+  const int64_t mt = (M + kTileM - 1) / kTileM, kb = (K + kScaleBlock - 1) / kScaleBlock;
+  const bool long_k = kb >= 32;
+  int tile_n = 256;
+  while (tile_n > 64 && (N <= tile_n / 2 || (!long_k && mt * ((N + tile_n - 1) / tile_n) < sms))) tile_n /= 2;
+  const int64_t tiles = mt * ((N + tile_n - 1) / tile_n);
+  int splits = 1;
+  if (long_k && 2 * tiles <= sms) splits = (int)std::min<int64_t>(sms / tiles, kb / 8);
+  return {tile_n, splits};
+}
+
+template <int kTileN, typename OutT>
+cudaError_t launch_matmul(const CUtensorMap &ma, const CUtensorMap &mb, MatmulArgs g, cudaStream_t s) {
+  static SmemGrant grant;
+  const cudaError_t e = grant.ensure(fp8_matmul_kernel<kTileN, OutT>, Shape<kTileN>::smem);
+  if (e != cudaSuccess) return e;
+  const int sms = sm_count();
+  const unsigned grid = (unsigned)(g.tiles < sms ? g.tiles : sms);
+  return launch_pdl(fp8_matmul_kernel<kTileN, OutT>, grid, (unsigned)Shape<kTileN>::threads, Shape<kTileN>::smem, s, ma, mb, g);
+}
+
+template <typename OutT>
+cudaError_t launch_matmul_n(int tile_n, const CUtensorMap &ma, const CUtensorMap &mb, const MatmulArgs &g, cudaStream_t s) {
+  if (tile_n == 256) return launch_matmul<256, OutT>(ma, mb, g, s);
+  if (tile_n == 128) return launch_matmul<128, OutT>(ma, mb, g, s);
+  return launch_matmul<64, OutT>(ma, mb, g, s);
+}
+
+template <typename OutT>
+cudaError_t launch_split_sum(const float *part, int splits, int64_t count, int N, const float *bias, void *out, cudaStream_t s) {
+  const int64_t blocks = (count + 255) / 256;
+  return launch_pdl(split_sum_kernel<OutT>, (unsigned)std::min<int64_t>(blocks, 16 * (int64_t)sm_count()), 256u, 0, s,
+                    part, splits, count, N, bias, static_cast<OutT *>(out));
+}
+
+template <typename T>
+cudaError_t launch_quantize(const void *x, const QuantArgs &a, int plain, int trans, cudaStream_t s) {
+  const unsigned grid = (unsigned)(a.row_tiles * a.col_tiles);
+  const T *p = static_cast<const T *>(x);
+  const bool sums = a.column_sums != nullptr;
+#define OTB_QUANT(P, R, S) \
+  if (plain == P && trans == R && sums == S) return launch_pdl(quantize_kernel<T, P, R, S>, grid, (unsigned)kQuantThreads, 0, s, p, a)
+  OTB_QUANT(kRowBlocks, kNone, false);
+  OTB_QUANT(kRowBlocks, kSquareBlocks, false);
+  OTB_QUANT(kSquareBlocks, kNone, false);
+  OTB_QUANT(kSquareBlocks, kSquareBlocks, false);
+  OTB_QUANT(kRowBlocks, kColumnBlocks, false);
+  OTB_QUANT(kRowBlocks, kColumnBlocks, true);
+#undef OTB_QUANT
+  return cudaErrorInvalidValue;
+}
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+}  // namespace otb
+
+using namespace otb;
+
+extern "C" {
+
+int ot_b200_fp8_quantize(const void *d_x, int64_t rows, int32_t cols, int64_t row_stride, uint32_t flags, int32_t mode,
+                         void *d_q, int64_t q_pitch, float *d_scale, void *d_qt, int64_t qt_pitch, float *d_scale_t,
+                         float *d_partial_sums, float *d_column_sums, void *stream) {
+  const uint32_t types = flags & (OT_B200_BF16 | OT_B200_FP16);
+  if ((flags & ~(OT_B200_BF16 | OT_B200_FP16)) || (types & (types - 1)))
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: flags may hold one of OT_B200_BF16 and OT_B200_FP16");
+  if (!d_x || rows <= 0 || cols <= 0 || rows > INT32_MAX || row_stride < cols)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: x is NULL or its sizes are not 1..2^31-1, or row_stride < cols");
+  if (mode < OT_B200_FP8_ROWS || mode > OT_B200_FP8_ROWS_AND_COLUMNS)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: unknown mode %d", mode);
+  const bool with_t = mode == OT_B200_FP8_ROWS_AND_SQUARES || mode == OT_B200_FP8_SQUARES_BOTH || mode == OT_B200_FP8_ROWS_AND_COLUMNS;
+  const int64_t need = (cols + 15) / 16 * 16, need_t = (rows + 15) / 16 * 16;
+  if (!d_q || !d_scale || !aligned16(d_q) || q_pitch % 16 != 0 || q_pitch < need)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: q and scale must be non-NULL, q 16-byte aligned, its pitch a multiple of 16 of at least cols");
+  if (with_t && (!d_qt || !d_scale_t || !aligned16(d_qt) || qt_pitch != need_t))
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: qt and scale_t must be non-NULL, qt 16-byte aligned, its pitch rows rounded up to 16");
+  if ((d_partial_sums == nullptr) != (d_column_sums == nullptr) || (d_column_sums && mode != OT_B200_FP8_ROWS_AND_COLUMNS))
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: column sums come with mode OT_B200_FP8_ROWS_AND_COLUMNS and both of their buffers");
+  QuantArgs a;
+  a.rows = rows;
+  a.ld = row_stride;
+  a.cols = cols;
+  a.col_tiles = (cols + kScaleBlock - 1) / kScaleBlock;
+  a.row_tiles = (rows + kScaleBlock - 1) / kScaleBlock;
+  if (a.row_tiles * a.col_tiles > INT32_MAX)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: more than 2^31 - 1 blocks of 128 x 128");
+  const size_t es = types ? 2 : 4;
+  a.vec = reinterpret_cast<uintptr_t>(d_x) % (4 * es) == 0 && row_stride % 4 == 0;
+  a.q = static_cast<uint8_t *>(d_q);
+  a.q_pitch = q_pitch;
+  a.scale = d_scale;
+  a.qt = static_cast<uint8_t *>(d_qt);
+  a.qt_pitch = qt_pitch;
+  a.scale_t = d_scale_t;
+  a.column_sums = d_partial_sums;
+  const int plain = (mode == OT_B200_FP8_SQUARES || mode == OT_B200_FP8_SQUARES_BOTH) ? kSquareBlocks : kRowBlocks;
+  const int trans = !with_t ? kNone : (mode == OT_B200_FP8_ROWS_AND_COLUMNS ? kColumnBlocks : kSquareBlocks);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (types == OT_B200_BF16) e = launch_quantize<__nv_bfloat16>(d_x, a, plain, trans, s);
+  else if (types == OT_B200_FP16) e = launch_quantize<__half>(d_x, a, plain, trans, s);
+  else e = launch_quantize<float>(d_x, a, plain, trans, s);
+  if (e == cudaSuccess && d_column_sums)
+    e = launch_pdl(column_sum_kernel, (unsigned)((cols + 7) / 8), 256u, 0, s, (const float *)d_partial_sums, a.row_tiles, (int)cols, d_column_sums);
+  if (e != cudaSuccess) return fail(OT_B200_ERR_CUDA, "ot_b200_fp8_quantize: %s", cudaGetErrorString(e));
+  return OT_B200_OK;
+}
+
+int ot_b200_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, uint64_t *bytes_out) {
+  if (!bytes_out || M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: sizes must be 1..2^31-1");
+  const MatmulPlan p = plan_matmul(M, N, K, sm_count());
+  *bytes_out = p.splits > 1 ? (uint64_t)p.splits * M * N * sizeof(float) : 0;
+  return OT_B200_OK;
+}
+
+int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a, const void *d_b, int64_t b_pitch,
+                       const float *d_scale_b, const float *d_bias, int64_t M, int64_t N, int64_t K, uint32_t flags,
+                       void *d_workspace, uint64_t workspace_bytes, void *d_out, void *stream) {
+  const uint32_t types = flags & (OT_B200_BF16 | OT_B200_FP16);
+  if ((flags & ~(OT_B200_BF16 | OT_B200_FP16 | OT_B200_REPORT_ERRORS)) || (types & (types - 1)))
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: flags may hold one of OT_B200_BF16 and OT_B200_FP16, and OT_B200_REPORT_ERRORS");
+  if (!d_a || !d_b || !d_scale_a || !d_scale_b || !d_out)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: NULL pointer");
+  if (!aligned16(d_a) || !aligned16(d_b) || a_pitch % 16 != 0 || b_pitch % 16 != 0 || a_pitch < K || b_pitch < K)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: operands must be 16-byte aligned, their pitches multiples of 16 of at least K");
+  uint64_t need = 0;
+  const int rc = ot_b200_fp8_matmul_workspace_bytes(M, N, K, &need);
+  if (rc) return rc;
+  const size_t es = types ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(d_out) % es != 0)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: out is not aligned to its type");
+  if (need > 0 && (!d_workspace || workspace_bytes < need || !aligned16(d_workspace)))
+    return fail(OT_B200_ERR_WORKSPACE, "ot_b200_fp8_matmul: workspace missing, misaligned or smaller than %llu bytes", (unsigned long long)need);
+  MatmulArgs g;
+  const int begun = begin_reported_call(flags, &g.sticky, &g.seq);
+  if (begun) return begun;
+  const MatmulPlan p = plan_matmul(M, N, K, sm_count());
+  CUtensorMap ma, mb;
+  if (!make_tensor_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, d_a, (uint64_t)M, (uint64_t)K, (uint64_t)a_pitch, kTileM, kScaleBlock) ||
+      !make_tensor_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, d_b, (uint64_t)N, (uint64_t)K, (uint64_t)b_pitch, (uint32_t)p.tile_n, kScaleBlock))
+    return fail(OT_B200_ERR_CUDA, "ot_b200_fp8_matmul: the driver's tensor-map encoder is not available or refused the operands");
+  g.sa = d_scale_a;
+  g.sb = d_scale_b;
+  g.M = M;
+  g.N = (int)N;
+  g.k_blocks = (int)((K + kScaleBlock - 1) / kScaleBlock);
+  g.n_tiles = (int)((N + p.tile_n - 1) / p.tile_n);
+  g.splits = p.splits;
+  g.tiles = (M + kTileM - 1) / kTileM * g.n_tiles * p.splits;
+  const bool split = p.splits > 1;
+  g.bias = split ? nullptr : d_bias;
+  g.out = static_cast<unsigned char *>(split ? d_workspace : d_out);
+  const uint64_t where = reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(N * (split ? sizeof(float) : es));
+  g.unit = where % 16 == 0 ? 16 : (where % 8 == 0 ? 8 : (where % 4 == 0 ? 4 : 2));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (split || types == 0) e = launch_matmul_n<float>(p.tile_n, ma, mb, g, s);
+  else if (types == OT_B200_BF16) e = launch_matmul_n<__nv_bfloat16>(p.tile_n, ma, mb, g, s);
+  else e = launch_matmul_n<__half>(p.tile_n, ma, mb, g, s);
+  if (e == cudaSuccess && split) {
+    const float *part = static_cast<const float *>(d_workspace);
+    if (types == 0) e = launch_split_sum<float>(part, p.splits, M * N, (int)N, d_bias, d_out, s);
+    else if (types == OT_B200_BF16) e = launch_split_sum<__nv_bfloat16>(part, p.splits, M * N, (int)N, d_bias, d_out, s);
+    else e = launch_split_sum<__half>(part, p.splits, M * N, (int)N, d_bias, d_out, s);
+  }
+  if (e != cudaSuccess) return fail(OT_B200_ERR_CUDA, "ot_b200_fp8_matmul: %s", cudaGetErrorString(e));
+  return OT_B200_OK;
+}
+
+}  // extern "C"

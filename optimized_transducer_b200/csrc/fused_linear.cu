@@ -34,9 +34,8 @@
 // records status word kStatusCopyTimeout, all roles leave their loops, the
 // producer waits (bounded) for its copies in flight, TMEM is freed and the CTA
 // returns.
-#include <cuda.h>  // CUtensorMap and its enums only; the encoder is looked up at run time
-
 #include "ot_common.cuh"
+#include "tensor_core.cuh"
 
 namespace otb {
 
@@ -59,41 +58,6 @@ constexpr uint32_t kBytesA = kTileM * kBlockK * 2;   // 16 KB
 constexpr uint32_t kBytesB = kTileN * kBlockK * 2;   // 32 KB
 constexpr uint32_t kStageBytes = kBytesA + kBytesB;  // 48 KB
 constexpr uint32_t kTmemColumns = 512;
-constexpr int kSpinLimit = 1 << 22;
-
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// Bounded wait; false when it ran out, or when another role of the CTA has given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, const volatile int *abort) {
-  for (int spin = 0; spin < kSpinLimit; ++spin) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((spin & 255) == 255 && *abort) return false;
-  }
-  return false;
-}
-
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int c0, int c1, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major operand tile whose rows are 128
-// bytes (64 bfloat16) in the 128-byte swizzle TMA writes: 8-row groups 1024 bytes
-// apart (stride byte offset), leading byte offset unused (1), descriptor version 1
-// (sm_100), layout type 2 (SWIZZLE_128B).  Addresses in units of 16 bytes.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);   // start address, bits [0,14)
-  d |= (uint64_t)1 << 16;                        // leading byte offset, bits [16,30)
-  d |= (uint64_t)(1024 >> 4) << 32;              // stride byte offset, bits [32,46)
-  d |= (uint64_t)1 << 46;                        // version, bits [46,48)
-  d |= (uint64_t)2 << 61;                        // layout type, bits [61,64)
-  return d;
-}
 
 // Instruction descriptor: float accumulator (bits [4,6) = 1), bfloat16 A and B
 // (bits [7,10) = [10,13) = 1), both K-major (bits 15, 16 = 0), N >> 3 at bit 17,
@@ -107,54 +71,6 @@ __device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t desc_a, uint6
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(kInstrDesc), "r"(accumulate)
-      : "memory");
-}
-
-// The mbarrier receives one arrival when every MMA issued so far has completed.
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// The same load without the wait, and the wait as a statement that "produces" the
-// registers, so that nothing that reads them can be scheduled above it.
-__device__ __forceinline__ void tmem_load_32_issue(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_load_32_wait(uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.wait::ld.sync.aligned;"
-      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-        "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-      :
       : "memory");
 }
 
@@ -545,51 +461,9 @@ linear_gradient_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     blank, nullptr, nullptr, GradArgs{coef, grad, d_scale, scale_host});
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-// The driver's tensor-map encoder, looked up through the runtime (the library
-// does not link libcuda).
-EncodeTiledFn encoder() {
-  static std::atomic<EncodeTiledFn> cached{nullptr};
-  EncodeTiledFn fn = cached.load(std::memory_order_acquire);
-  if (fn == nullptr) {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    fn = reinterpret_cast<EncodeTiledFn>(p);
-    cached.store(fn, std::memory_order_release);
-  }
-  return fn;
-}
-
-// (outer, inner) bfloat16 matrix, row-major; boxes of box_outer x 64 elements, 128-byte swizzle.
+// (outer, inner) bfloat16 matrix, row-major; boxes of box_outer x 64 elements.
 bool make_map(CUtensorMap *map, const void *base, uint64_t outer, uint64_t inner, uint32_t box_outer) {
-  EncodeTiledFn fn = encoder();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {inner * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kBlockK, box_outer};
-  const cuuint32_t elem[2] = {1, 1};
-  const auto encode = [&]() {
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, elem,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  CUresult r = encode();
-  if (r == CUDA_ERROR_INVALID_CONTEXT) {
-    // The encoder is a driver call and wants the device's context current on this
-    // thread.  A thread that has only been handed cached memory so far (an autograd
-    // worker whose first job is a small batch) has made no runtime call that binds
-    // it: bind it the way the runtime does for its own calls, and ask again.
-    (void)cudaFree(nullptr);
-    r = encode();
-  }
-  return r == CUDA_SUCCESS;
+  return make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, outer, inner, inner * 2, box_outer, kBlockK);
 }
 
 }  // namespace

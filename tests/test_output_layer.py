@@ -1,0 +1,60 @@
+"""What the output-layer entry points refuse, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import optimized_transducer_b200 as ot
+from optimized_transducer_b200 import _lib
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(2, 16), torch.zeros(3, 16)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ot.joiner_logits(x, w)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ot.quantize_weight(w)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ot.Fp8Weight(w.to(torch.float8_e4m3fn), torch.ones(1, 1))
+    with pytest.raises(RuntimeError, match="float8_e4m3fn"):
+        ot.Fp8Weight(w, torch.ones(1, 1))
+
+
+def _memory():
+    buf = ctypes.create_string_buffer(4096)
+    return buf, (ctypes.addressof(buf) + 255) & ~255
+
+
+def test_quantiser_argument_errors():
+    lib = _lib.load()
+    keep, p = _memory()
+
+    def call(x=p, rows=4, cols=20, ld=20, flags=0, mode=_lib.FP8_ROWS, q=p, pitch=32, s=p, qt=None, tp=0, st=None, part=None, tot=None):
+        return lib.ot_b200_fp8_quantize(x, rows, cols, ld, flags, mode, q, pitch, s, qt, tp, st, part, tot, None)
+
+    bad = [dict(x=None), dict(rows=0), dict(cols=0), dict(rows=1 << 31), dict(ld=19), dict(flags=_lib.FP64),
+           dict(flags=_lib.BF16 | _lib.FP16), dict(mode=5), dict(mode=-1), dict(q=None), dict(q=p + 8), dict(pitch=20), dict(pitch=16),
+           dict(s=None), dict(mode=_lib.FP8_SQUARES_BOTH), dict(mode=_lib.FP8_SQUARES_BOTH, qt=p, tp=32, st=p),
+           dict(part=p, tot=p), dict(mode=_lib.FP8_ROWS_AND_COLUMNS, qt=p, tp=16, st=p, part=p)]
+    for kw in bad:
+        assert call(**kw) == _lib.ERR_ARGUMENT, kw
+        assert "ot_b200_fp8_quantize" in _lib.last_error()
+
+
+def test_product_argument_errors():
+    lib = _lib.load()
+    keep, p = _memory()
+
+    def call(a=p, ap=32, sa=p, b=p, bp=32, sb=p, M=4, N=5, K=20, flags=0, ws=None, wb=0, out=p):
+        return lib.ot_b200_fp8_matmul(a, ap, sa, b, bp, sb, None, M, N, K, flags, ws, wb, out, None)
+
+    bad = [dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(out=None), dict(a=p + 8), dict(b=p + 1), dict(ap=24),
+           dict(bp=16), dict(M=0), dict(N=0), dict(K=0), dict(M=1 << 31), dict(flags=_lib.FP64), dict(out=p + 2)]
+    for kw in bad:
+        assert call(**kw) == _lib.ERR_ARGUMENT, kw
+    long_k = dict(M=10, N=10, K=100000, ap=100000, bp=100000)
+    assert call(**long_k) == _lib.ERR_WORKSPACE
+    need = ctypes.c_uint64()
+    assert lib.ot_b200_fp8_matmul_workspace_bytes(10, 10, 100000, ctypes.byref(need)) == _lib.OK and need.value > 0
+    assert call(**long_k, ws=p, wb=need.value - 1) == _lib.ERR_WORKSPACE
+    assert lib.ot_b200_fp8_matmul_workspace_bytes(100000, 500, 512, ctypes.byref(need)) == _lib.OK and need.value == 0
