@@ -342,6 +342,48 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
                        int64_t N, int64_t K, uint32_t flags, void *d_workspace,
                        uint64_t workspace_bytes, void *d_out, void *stream);
 
+/* One symbol per row of logits (rows, V; unit column stride, rows row_stride elements
+ * apart; float, or as OT_B200_BF16 / OT_B200_FP16 in `flags` says), from the uniform
+ * numbers d_uniforms (rows, in [0, 1]).  With w_i = exp((x_i - max x) / temperature):
+ *   top_k   keeps the k largest logits (k <= 0 or k >= V: all of them)
+ *   top_p   keeps, of what is left, every i before which the weights sum to less than
+ *           top_p times what is left weighs (top_p >= 1: all, top_p <= 0: the first)
+ *   min_p   keeps, of what is left, every i with w_i >= min_p, and the first (0: all)
+ *   d_tokens[r]    the first index, in index order, at which the kept weights sum to
+ *                  more than u times their total (u = 1: the last kept one)
+ *   d_logprobs[r]  log of its weight over that total
+ * "Before" and "first" are in the order of falling logits, the lower index first among
+ * equal ones.  temperature 0 takes the first (log-probability 0).  The tokens are those of
+ * the definition in 64-bit arithmetic.  -inf logits are never drawn.  A row without a finite
+ * maximum (all -inf, or one NaN or +inf in it), or with u, temperature, top_p or min_p that
+ * is a NaN or out of range (u in [0, 1], temperature in [0, 1e6]) gets token -1 and
+ * log-probability NaN.  Each setting is one per row (d_... not NULL) or the scalar. */
+#define OT_B200_SAMPLE_MAX_V 262144
+int ot_b200_sample(const void *d_logits, int64_t rows, int32_t V, int64_t row_stride, uint32_t flags,
+                   const float *d_uniforms, const float *d_temperature, float temperature,
+                   const int32_t *d_top_k, int32_t top_k, const float *d_top_p, float top_p,
+                   const float *d_min_p, float min_p, int32_t *d_tokens, float *d_logprobs,
+                   void *stream);
+
+/* The norm of n gradients together and clipping by it, as torch.nn.utils.clip_grad_norm_
+ * defines it:  norm = (sum |g|^p)^(1/p) over all elements of all tensors,
+ *   out = g * min(1, max_norm / (norm + 1e-6)).
+ * Host arrays of n entries: device pointers, element counts (0 is skipped) and element
+ * types (0 float, OT_B200_FP64, OT_B200_BF16, OT_B200_FP16; they may differ).  outs /
+ * out_types: where the clipped gradients go, or NULL: in place; with every output in
+ * place nothing is written when the factor is 1.  Tensors must not overlap (one listed
+ * twice is refused), nor an output another tensor.  apply = 0: only the norm.
+ * *d_norm (float) receives the norm; sums are taken in double over groups of at most 32
+ * elements, in a fixed order.  A norm that is not finite scales as it does in torch
+ * (infinite: by 0; NaN: by NaN).  The workspace (8-byte aligned) may be reused by the next
+ * call on the same stream.  Callable in a stream capture; nothing is copied to the device. */
+typedef enum ot_b200_norm_kind { OT_B200_NORM_INF = 0, OT_B200_NORM_1 = 1, OT_B200_NORM_2 = 2 } ot_b200_norm_kind;
+int ot_b200_clip_workspace_bytes(int32_t n, uint64_t *bytes_out);
+int ot_b200_clip_gradients(int32_t n, const void *const *grads, const int64_t *counts, const int32_t *types,
+                           void *const *outs, const int32_t *out_types, int32_t norm_kind, int32_t apply,
+                           double max_norm, void *d_workspace, uint64_t workspace_bytes, float *d_norm,
+                           void *stream);
+
 /* d_grad[i] *= *d_scale for i < count, unless *d_scale == 1 (then the buffer is
  * not touched: the kernel's blocks return after one load).  The counterpart of
  * `ctx.grad.mul_(loss_grad)` (transducer_loss.py:162) for a gradient that

@@ -28,6 +28,9 @@ TRACE = 512
 REPORT_ERRORS = 1024
 LINEAR_DOMAIN = 2048
 
+# ot_b200_norm_kind
+NORM_INF, NORM_1, NORM_2 = range(3)
+
 # ot_b200_fp8_mode
 (FP8_ROWS, FP8_SQUARES, FP8_ROWS_AND_SQUARES, FP8_SQUARES_BOTH, FP8_ROWS_AND_COLUMNS) = range(5)
 
@@ -44,6 +47,9 @@ EXPORTS = (
     "ot_b200_scale_gradient",
     "ot_b200_forward_linear",
     "ot_b200_backward_linear",
+    "ot_b200_sample",
+    "ot_b200_clip_workspace_bytes",
+    "ot_b200_clip_gradients",
     "ot_b200_fp8_quantize",
     "ot_b200_fp8_matmul_workspace_bytes",
     "ot_b200_fp8_matmul",
@@ -112,6 +118,13 @@ def load():
     lib.ot_b200_backward_linear.restype = ctypes.c_int
     lib.ot_b200_backward_linear.argtypes = [vp, vp, vp, i32, i64, i32, i32, i32, i32, u32, vp, u64, vp, vp,
                                             ctypes.c_double, vp]
+    f32 = ctypes.c_float
+    lib.ot_b200_sample.restype = ctypes.c_int
+    lib.ot_b200_sample.argtypes = [vp, i64, i32, i64, u32, vp, vp, f32, vp, i32, vp, f32, vp, f32, vp, vp, vp]
+    lib.ot_b200_clip_workspace_bytes.restype = ctypes.c_int
+    lib.ot_b200_clip_workspace_bytes.argtypes = [i32, ctypes.POINTER(u64)]
+    lib.ot_b200_clip_gradients.restype = ctypes.c_int
+    lib.ot_b200_clip_gradients.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, ctypes.c_double, vp, u64, vp, vp]
     lib.ot_b200_fp8_quantize.restype = ctypes.c_int
     lib.ot_b200_fp8_quantize.argtypes = [vp, i64, i32, i64, u32, i32, vp, i64, vp, vp, i64, vp, vp, vp, vp]
     lib.ot_b200_fp8_matmul_workspace_bytes.restype = ctypes.c_int

@@ -69,23 +69,6 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   return lo | (hi << 16);
 }
 
-template <typename T> __device__ __forceinline__ float to_float(T x) { return (float)x; }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-
-template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]);
-template <> __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
-  const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-}
-template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]) {
-  const uint2 a = __ldg(reinterpret_cast<const uint2 *>(p));
-  T t[4];
-  memcpy(t, &a, sizeof(a));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = to_float(t[i]);
-}
-
 enum { kNone = 0, kRowBlocks = 1, kSquareBlocks = 2, kColumnBlocks = 1 };
 
 struct QuantArgs {

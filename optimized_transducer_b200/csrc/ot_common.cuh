@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 #include <atomic>
 
@@ -380,6 +381,24 @@ template <> struct Pair16<__half> {
   }
 };
 #endif
+
+// Element conversion, and four consecutive elements at once (p aligned to all four).
+template <typename T> __device__ __forceinline__ float to_float(T x) { return (float)x; }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]);
+template <> __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
+  const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]) {
+  const uint2 a = __ldg(reinterpret_cast<const uint2 *>(p));
+  T t[4];
+  memcpy(t, &a, sizeof(a));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = to_float(t[i]);
+}
 
 template <typename T> __device__ __forceinline__ T neg_inf();
 template <> __device__ __forceinline__ float neg_inf<float>() { return -__int_as_float(0x7f800000); }
