@@ -1,4 +1,5 @@
-"""Builds ``libot_b200.so`` (the sm_100a kernels + the C ABI) in-tree with nvcc.
+"""Builds ``libot_b200.so`` (the sm_100a kernels + the C ABI) in-tree with nvcc, and
+``_tensors.so``, a small helper of the Python layer, with g++ against torch's headers.
 
 Usage: ``python -m optimized_transducer_b200.build [-v]``.  The library links
 the CUDA runtime statically and has no dependency on torch or Python.
@@ -7,10 +8,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libot_b200.so")
+HELPER = os.path.join(HERE, "_tensors.so")
+HELPER_SOURCE = os.path.join(CSRC, "tensors.cc")
 SOURCES = ["api.cu", "prep.cu", "logprob.cu", "lattice.cu", "gradient.cu", "noalloc.cu", "pack.cu",
            "exchange.cu", "fused_linear.cu", "fp8.cu", "sample.cu", "clip.cu"]
 HEADERS = [os.path.join(CSRC, "ot_common.cuh"), os.path.join(CSRC, "tensor_core.cuh"),
@@ -33,8 +37,39 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in deps)
 
 
+def start_helper():
+    """Starts the compilation of ``_tensors.so``."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], cuda)], HELPER_SOURCE, "-o", HELPER,
+           f"-L{libs}", "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def finish_helper(proc, verbose=False):
+    out, _ = proc.communicate()
+    if verbose or proc.returncode != 0:
+        sys.stderr.write(out)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed on {HELPER_SOURCE}")
+
+
 def build(force=False, verbose=False):
     """Compiles every kernel for sm_100a; returns the path of the library."""
+    newest = max(os.path.getmtime(HELPER_SOURCE), os.path.getmtime(HEADERS[-1]))
+    helper = start_helper() if force or not os.path.isfile(HELPER) or os.path.getmtime(HELPER) < newest else None
+    try:
+        return build_library(force, verbose)
+    finally:
+        if helper is not None:
+            finish_helper(helper, verbose)
+
+
+def build_library(force=False, verbose=False):
     if not force and up_to_date():
         return LIB
     nvcc = nvcc_path()

@@ -10,75 +10,78 @@ import math
 import torch
 
 from . import _lib
-from .transducer_loss import _DTYPE_FLAG, _on_device
+from .transducer_loss import _on_device
 
 __all__ = ["grad_norm", "clip_grad_norm_"]
 
 _KINDS = {1.0: _lib.NORM_1, 2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
 
 
-def _dense(t):
-    """Whether t fills one stretch of memory, each element once (any order of its dimensions)."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((t.stride(d), t.size(d)) for d in range(t.dim()) if t.size(d) != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
+_helper = None
 
 
-def _table(tensors, who, what, device):
-    """(pointers, counts, type flags) of dense CUDA tensors on one device, as ctypes arrays."""
-    n = len(tensors)
-    try:
-        types = [_DTYPE_FLAG[t.dtype] for t in tensors]
-    except KeyError as e:
-        raise RuntimeError(f"{who}: expected {what} to be float32, float64, bfloat16 or float16, got {e.args[0]}") from None
-    for t in tensors:
-        if t.get_device() != device:
-            raise RuntimeError(f"{who}: expected {what} to be CUDA tensors on one device (sm_100a kernels, no CPU path), "
-                               f"got one on {t.device}")
-        if t.layout != torch.strided or not (t.is_contiguous() or _dense(t)):
-            raise RuntimeError(f"{who}: expected {what} to be dense (no gaps, no expanded dimensions), got "
-                               f"{t.layout} of shape {tuple(t.shape)}")
-    counts = [t.numel() for t in tensors]
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]), (ctypes.c_int64 * n)(*counts),
-            (ctypes.c_int32 * n)(*types))
+def _tensors():
+    """The compiled helper that reads a list of tensors in one call."""
+    global _helper
+    if _helper is None:
+        try:
+            from . import _tensors as helper
+        except ImportError as e:
+            raise ImportError("optimized_transducer_b200/_tensors.so is missing or does not load: build it with "
+                              f"`python -m optimized_transducer_b200.build` ({e})") from None
+        _helper = helper
+    return _helper
+
+
+def _table(tensors, who, what):
+    """(pointers, counts, type flags, device) of dense CUDA tensors on one device; the first three are C arrays."""
+    pointers, counts, types, device, at, why = _tensors().describe(tensors)
+    if why == "":
+        return pointers, counts, types, device
+    t = tensors[at]
+    if why == "tensor":
+        raise RuntimeError(f"{who}: expected {what} to be tensors, got {type(t).__name__}")
+    if why == "type":
+        raise RuntimeError(f"{who}: expected {what} to be float32, float64, bfloat16 or float16, got {t.dtype}")
+    if why == "layout":
+        raise RuntimeError(f"{who}: expected {what} to be dense (no gaps, no expanded dimensions), got {t.layout} of shape "
+                           f"{tuple(t.shape)}")
+    if why == "cpu":
+        raise RuntimeError(f"{who}: CUDA tensors only (sm_100a kernels, no CPU path), got one on {t.device}")
+    raise RuntimeError(f"{who}: expected {what} to be on one device, got {t.device} and {tensors[0].device}")
 
 
 def _call(who, tensors, norm_type, apply, max_norm, out):
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     kind = _KINDS.get(float(norm_type))
     if kind is None:
         raise RuntimeError(f"{who}: norm_type must be 1, 2 or inf, got {norm_type}")
     if not tensors:
         raise RuntimeError(f"{who}: no gradients were given")
-    device = tensors[0].get_device()
-    if device < 0:
-        raise RuntimeError(f"{who}: CUDA tensors only (sm_100a kernels, no CPU path)")
-    grads, counts, types = _table(tensors, who, "the gradients", device)
+    grads, counts, types, device = _table(tensors, who, "the gradients")
     outs = out_types = None
     if out is not None:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(tensors):
             raise RuntimeError(f"{who}: expected one output per gradient, got {len(out)} for {len(tensors)}")
-        for t, o in zip(tensors, out):
-            if t.shape != o.shape or (t.stride() != o.stride() and not (t.is_contiguous() and o.is_contiguous())):
-                raise RuntimeError(f"{who}: an output must have its gradient's shape and strides, got {tuple(o.shape)} "
-                                   f"for {tuple(t.shape)}")
-        outs, _, out_types = _table(out, who, "the outputs", device)
+        outs, _, out_types, out_device = _table(out, who, "the outputs")
+        at = _tensors().alike(tensors, out)
+        if at >= 0 or out_device != device:
+            raise RuntimeError(f"{who}: an output must have its gradient's shape, strides and device, got {tuple(out[at].shape)} "
+                               f"on {out[at].device} for {tuple(tensors[at].shape)} on {tensors[at].device}")
     lib = _lib.load()
+    n = len(tensors)
     with _on_device(device):
         need = ctypes.c_uint64()
-        _lib.check(lib.ot_b200_clip_workspace_bytes(len(tensors), ctypes.byref(need)))
+        _lib.check(lib.ot_b200_clip_workspace_bytes(n, ctypes.byref(need)))
         ws = torch.empty(need.value, dtype=torch.uint8, device=tensors[0].device)
         norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
         _lib.check(lib.ot_b200_clip_gradients(
-            len(tensors), grads, counts, types, outs, out_types, kind, 1 if apply else 0, float(max_norm), ws.data_ptr(),
+            n, grads, counts, types, outs, out_types, kind, 1 if apply else 0, float(max_norm), ws.data_ptr(),
             need.value, norm.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
     return norm
+
+
+def _list(tensors):
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
 
 
 def grad_norm(tensors, norm_type=2.0):
@@ -87,7 +90,7 @@ def grad_norm(tensors, norm_type=2.0):
     tensor or an iterable of them, float32, float64, bfloat16 or float16, mixed as one
     likes.  Sums are taken in float64 over groups of at most 32 elements in a fixed
     order: the same inputs give the same bits."""
-    return _call("grad_norm", tensors, norm_type, False, 0.0, None)
+    return _call("grad_norm", _list(tensors), norm_type, False, 0.0, None)
 
 
 def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
@@ -103,8 +106,8 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
     who = "clip_grad_norm_"
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"{who}: max_norm must not be negative or a NaN, got {max_norm}")
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    written = tensors if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
+    tensors = _list(tensors)
+    written = tensors if out is None else _list(out)
     norm = _call(who, tensors, norm_type, True, max_norm, None if out is None else written)
-    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    _tensors().written(written)
     return norm

@@ -74,7 +74,7 @@ enum { kNone = 0, kRowBlocks = 1, kSquareBlocks = 2, kColumnBlocks = 1 };
 struct QuantArgs {
   int64_t rows, ld;     // ld: elements from one row of x to the next
   int cols, col_tiles;
-  bool vec;             // every group of four columns may be loaded at once
+  bool vec;             // four columns may be loaded at once, and their number is a multiple of four
   uint8_t *q;           // (rows, cols), rows q_pitch bytes apart
   int64_t q_pitch;
   float *scale;         // kRowBlocks: [column tile][row]; kSquareBlocks: [row tile][column tile]
@@ -105,20 +105,23 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
   pdl_trigger();
 
   float v[kQuantRows][4];
+  if (a.vec) {
+    // groups of four lie inside a row or outside; all loads are requested before one is used
+    typename Raw4<T>::type raw[kQuantRows];
+    const T *p = x + row0 * a.ld + col;
 #pragma unroll
-  for (int i = 0; i < kQuantRows; ++i) {
-    const int64_t row = row0 + i;
-    const T *p = x + row * a.ld + col;
-    v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
-    if (row < a.rows) {
-      if (a.vec && col + 3 < a.cols) {
-        load4<T>(p, v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < a.cols) v[i][j] = to_float(p[j]);
-      }
+    for (int i = 0; i < kQuantRows; ++i) {
+      raw[i] = typename Raw4<T>::type{};
+      if (row0 + i < a.rows && col < a.cols) raw[i] = load4(p + i * a.ld);
     }
+#pragma unroll
+    for (int i = 0; i < kQuantRows; ++i) convert4<T>(raw[i], v[i]);
+  } else {
+    const T *p = x + row0 * a.ld + col;
+#pragma unroll
+    for (int i = 0; i < kQuantRows; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = row0 + i < a.rows && col + j < a.cols ? to_float(__ldg(p + i * a.ld + j)) : 0.f;
   }
 
   if constexpr (kPlain == kRowBlocks) {
@@ -249,17 +252,19 @@ column_sum_kernel(const float *__restrict__ part, int64_t row_tiles, int cols, f
 constexpr int kTileM = 128;                      // rows per tile = TMEM lanes
 constexpr int kMmaK = 32;                        // K of one tcgen05.mma for 8-bit operands
 constexpr uint32_t kBytesA = kTileM * kScaleBlock;
-constexpr int kStagePitch = 80;                  // bytes from row to row of a warp's 32 x 64-byte staging tile
+constexpr int kStagedBytes = 32 * 128;           // a warp's staging tile: 32 rows of 128 bytes in the 128-byte swizzle
 
-// Columns per tile: 256, 128 or 64.  Every epilogue warp owns 32 rows x 64 columns.
+// Columns per tile: 256, 128 or 64.  An epilogue warp owns 32 rows x `columns` columns.
 template <int kTileN> struct Shape {
-  static constexpr int epilogue_warps = kTileN / 16;
+  static constexpr int columns = kTileN == 256 ? 128 : 64;
+  static constexpr int epilogue_warps = 4 * kTileN / columns;
   static constexpr int threads = 64 + 32 * epilogue_warps;
   static constexpr uint32_t stage_bytes = kBytesA + kTileN * kScaleBlock;
-  static constexpr int ring = kTileN == 256 ? 3 : (kTileN == 128 ? 5 : 6);
+  static constexpr int ring = kTileN == 256 ? 3 : (kTileN == 128 ? 4 : 6);
   static constexpr int accumulators = kTileN == 256 ? 2 : 4;
+  static constexpr int staged_tiles = columns / 64;  // tiles per warp: its columns in 16 bits, half of them in float
   static constexpr uint32_t tmem_columns = accumulators * kTileN;
-  static constexpr size_t smem = 1024 + (size_t)ring * stage_bytes + (size_t)epilogue_warps * 32 * kStagePitch;
+  static constexpr size_t smem = 1024 + (size_t)ring * stage_bytes + (size_t)epilogue_warps * staged_tiles * kStagedBytes;
   // kind::f8f6f4: float accumulator (bits [4,6) = 1), e4m3 A and B (0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24
   static constexpr uint32_t instr = (1u << 4) | ((uint32_t)(kTileN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
 };
@@ -291,33 +296,45 @@ __device__ __forceinline__ void tmem_load_16_wait(uint32_t (&r)[16]) {
       : "memory");
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);  // 16-bit types
-template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) { return Pair16<__nv_bfloat16>::round(a, b); }
-template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) { return Pair16<__half>::round(a, b); }
+// Rounds two floats to a pair of 16-bit values (not called for float).
+template <typename T> __device__ __forceinline__ uint32_t round_pair(float a, float b) { return Pair16<T>::round(a, b); }
 
-// Copies a staged 32-row x 64-byte tile to rows of out that are `pitch` bytes apart, in
-// units of sizeof(U) bytes: a store instruction covers whole pieces of rows.
+// Where 16-byte piece `piece` of row `row` of a staging tile lies (128-byte swizzle: what a
+// TMA store expects; also, a warp that writes or reads a column of pieces hits every bank once).
+__device__ __forceinline__ int staged_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// Copies a staged tile to rows of out that are `pitch` bytes apart, in units of sizeof(U)
+// bytes: a store instruction covers whole 128-byte pieces of rows.
 template <typename U>
 __device__ __forceinline__ void store_staged(const unsigned char *staged, unsigned char *out, int64_t pitch, int rows, int bytes, int lane) {
-  constexpr int kUnits = 64 / sizeof(U);                 // units per row
+  constexpr int kUnits = 128 / sizeof(U);                // units per row
   constexpr int kRows = kUnits >= 32 ? 1 : 32 / kUnits;  // rows per instruction
-  const int unit = lane % kUnits, r0 = lane / kUnits;
-  if (unit * (int)sizeof(U) >= bytes) return;
+#pragma unroll
+  for (int u0 = 0; u0 < kUnits; u0 += 32) {
+    const int unit = u0 + lane % kUnits, r0 = lane / kUnits, byte = unit * (int)sizeof(U);
+    if (byte < bytes) {
+      unsigned char *dst = out + r0 * pitch + byte;
 #pragma unroll 4
-  for (int r = r0; r < rows; r += kRows)
-    *reinterpret_cast<U *>(out + r * pitch + unit * sizeof(U)) =
-        *reinterpret_cast<const U *>(staged + r * kStagePitch + unit * sizeof(U));
+      for (int r = r0; r < rows; r += kRows, dst += kRows * pitch)
+        *reinterpret_cast<U *>(dst) = *reinterpret_cast<const U *>(staged + staged_at(r, byte >> 4) + (byte & 15));
+    }
+  }
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
 }
 
 struct MatmulArgs {
   const float *sa;      // [K block][M]
   const float *sb;      // [N / 128][K block]
   const float *bias;    // [N] or NULL
-  unsigned char *out;   // (splits, M, N): splits > 1 holds partial sums
-  int64_t M;
+  unsigned char *out;   // (M, N); pieces of K: (splits, out_rows, N) partial sums
+  int64_t M, out_rows;
   int N, k_blocks, n_tiles, splits;
-  int64_t tiles;
-  int unit;             // bytes per store: the largest of 16, 8, 4, 2 that divides the rows' pitch and the base
+  uint32_t tiles;
+  int unit;             // bytes per store, the largest of 8, 4, 2 that divides the rows' pitch and the base; 0: TMA stores (16 bytes do)
   int32_t *sticky;      // error record, or NULL
   int32_t seq;
 };
@@ -326,19 +343,18 @@ template <int kTileN> struct MatmulShared {
   uint64_t full[Shape<kTileN>::ring];          // TMA -> MMA
   uint64_t empty[Shape<kTileN>::ring];         // MMA -> TMA
   uint64_t acc_full[Shape<kTileN>::accumulators];   // MMA -> epilogue: one K block's product is complete
-  uint64_t acc_empty[Shape<kTileN>::accumulators];  // epilogue -> MMA
+  uint64_t acc_empty[Shape<kTileN>::accumulators];  // epilogue -> MMA, one arrival per warp: 256 of them took as long as the block's MMAs
   uint32_t tmem_base;
   int never;
   volatile int abort;
-  alignas(16) float bias[Shape<kTileN>::epilogue_warps][64];  // read as float4
+  alignas(16) float bias[Shape<kTileN>::epilogue_warps][Shape<kTileN>::columns];  // read as float4
 };
 
 // One CTA per SM, persistent over (row tile, column tile, piece of K).  The scales change
 // with every K block, so a block's product is complete in tensor memory on its own (four
 // MMAs of K = 32) and the epilogue adds it, scaled, to sums held in registers in float:
 // one multiply-add per element and K block, which runs while the tensor cores work on the
-// next block's product.  Per K block the MMAs take kTileN * 2 cycles; the sixteen epilogue
-// warps of the widest tile need 64 multiply-adds and four 16-column reads each.
+// next block's product.
 //   warp 0   TMA producer: a (128 x 128) and b (kTileN x 128) boxes into the ring
 //   warp 1   MMA issuer
 //   others   epilogue: warp % 4 picks the TMEM lanes (rows), the rest the 64 columns
@@ -346,7 +362,8 @@ template <int kTileN> struct MatmulShared {
 // (bounded) for its copies in flight, and the record of the failure goes to `sticky`.
 template <int kTileN, typename OutT>
 __global__ void __launch_bounds__(Shape<kTileN>::threads, 1)
-fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MatmulArgs g) {
+fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const __grid_constant__ CUtensorMap map_out, const MatmulArgs g) {
   using S = Shape<kTileN>;
   constexpr int R = S::ring, B = S::accumulators;
   extern __shared__ __align__(1024) unsigned char ring_mem[];
@@ -357,7 +374,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < R; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
-    for (int i = 0; i < B; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], 32 * S::epilogue_warps); }
+    for (int i = 0; i < B; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], S::epilogue_warps); }
     sh.abort = 0;
     sh.never = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -377,29 +394,36 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
   // tile -> (piece of K, row tile, column tile), the column tile fastest: the row tile's
   // bytes are read once from HBM and again from L2
-  const auto place = [&](int64_t tile, int &nt, int64_t &mt, int &sp, int &k0, int &k1) {
-    nt = (int)(tile % g.n_tiles);
-    const int64_t rest = tile / g.n_tiles;
-    sp = (int)(rest % g.splits);
-    mt = rest / g.splits;
-    k0 = (int)((int64_t)g.k_blocks * sp / g.splits);
-    k1 = (int)((int64_t)g.k_blocks * (sp + 1) / g.splits);
+  struct Place { int nt, mt, sp, k0, k1; };
+  const auto place = [&](uint32_t tile) {
+    const uint32_t rest = tile / (uint32_t)g.n_tiles;
+    Place p;
+    p.nt = (int)(tile - rest * (uint32_t)g.n_tiles);
+    p.mt = (int)rest;
+    p.sp = 0;
+    p.k0 = 0;
+    p.k1 = g.k_blocks;
+    if (g.splits > 1) {
+      p.mt = (int)(rest / (uint32_t)g.splits);
+      p.sp = (int)rest - p.mt * g.splits;
+      p.k0 = (int)((int64_t)g.k_blocks * p.sp / g.splits);
+      p.k1 = (int)((int64_t)g.k_blocks * (p.sp + 1) / g.splits);
+    }
+    return p;
   };
 
   if (warp == 0 && lane == 0) {
     uint32_t it = 0;
-    for (int64_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
-      int nt, sp, k0, k1;
-      int64_t mt;
-      place(tile, nt, mt, sp, k0, k1);
-      for (int kb = k0; kb < k1; ++kb, ++it) {
+    for (uint32_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
+      const Place p = place(tile);
+      for (int kb = p.k0; kb < p.k1; ++kb, ++it) {
         const int s = it % R;
         if (it >= R && !mbar_wait(&sh.empty[s], ((it / R) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
         unsigned char *a = ring + (size_t)s * S::stage_bytes;
         mbar_expect_tx(&sh.full[s], S::stage_bytes);
         // what lies beyond either matrix is filled with zeros by the copy
-        tma_load_2d(a, &map_a, kb * kScaleBlock, (int)(mt * kTileM), &sh.full[s]);
-        tma_load_2d(a + kBytesA, &map_b, kb * kScaleBlock, nt * kTileN, &sh.full[s]);
+        tma_load_2d(a, &map_a, kb * kScaleBlock, p.mt * kTileM, &sh.full[s]);
+        tma_load_2d(a + kBytesA, &map_b, kb * kScaleBlock, p.nt * kTileN, &sh.full[s]);
       }
     }
     if (sh.abort) {
@@ -415,11 +439,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
   } else if (warp == 1 && lane == 0) {
     uint32_t it = 0;
-    for (int64_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
-      int nt, sp, k0, k1;
-      int64_t mt;
-      place(tile, nt, mt, sp, k0, k1);
-      for (int kb = k0; kb < k1; ++kb, ++it) {
+    for (uint32_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
+      const Place p = place(tile);
+      for (int kb = p.k0; kb < p.k1; ++kb, ++it) {
         const int s = it % R, buf = it % B;
         if (it >= B && !mbar_wait(&sh.acc_empty[buf], ((it / B) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
         if (!mbar_wait(&sh.full[s], (it / R) & 1, &sh.abort)) { sh.abort = 1; break; }
@@ -436,89 +458,136 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   } else if (warp >= 2) {
     const int quarter = warp & 3;
     const int part = (warp - 2) >> 2;
-    unsigned char *staged = staging + (size_t)(warp - 2) * 32 * kStagePitch;
+    constexpr int kCols = S::columns;
+    unsigned char *staging_tiles = staging + (size_t)(warp - 2) * S::staged_tiles * kStagedBytes;
+    float *bias_s = sh.bias[warp - 2];
     uint32_t it = 0;
     bool dead = false;  // the same for all lanes: the reads of tensor memory are warp-wide
-    for (int64_t tile = blockIdx.x; tile < g.tiles && !dead; tile += gridDim.x) {
-      int nt, sp, k0, k1;
-      int64_t mt;
-      place(tile, nt, mt, sp, k0, k1);
-      const int64_t row0 = mt * kTileM + quarter * 32;
-      const int64_t row = row0 + lane;
-      const int col0 = nt * kTileN + part * 64;
-      const bool live = row < g.M;
-      const float *sa = g.sa + (live ? row : 0);
-      const float *sb = g.sb + (int64_t)min(col0 / kScaleBlock, (g.N - 1) / kScaleBlock) * g.k_blocks;
-      __syncwarp();  // the previous tile's bias has been read
-      sh.bias[warp - 2][lane] = (g.bias != nullptr && col0 + lane < g.N) ? __ldg(g.bias + col0 + lane) : 0.f;
-      sh.bias[warp - 2][lane + 32] = (g.bias != nullptr && col0 + 32 + lane < g.N) ? __ldg(g.bias + col0 + 32 + lane) : 0.f;
-      float acc[64];
+    // The scales of the next K block and the bias of the next tile are requested one block
+    // ahead, across tiles: a load's latency is longer than a block's multiply-adds.
+    const float *sa = nullptr, *sb = nullptr;
+    float sa_next = 0.f, sb_next = 0.f, bias_next[kCols / 32];
+    const auto aim = [&](const Place &p) {
+      const int64_t row = (int64_t)p.mt * kTileM + quarter * 32 + lane;
+      const int col0 = p.nt * kTileN + part * kCols;
+      sa = g.sa + (int64_t)p.k0 * g.M + (row < g.M ? row : 0);
+      sb = g.sb + (int64_t)min(col0 / kScaleBlock, (g.N - 1) / kScaleBlock) * g.k_blocks + p.k0;
+      sa_next = __ldg(sa);
+      sb_next = __ldg(sb);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = 0.f;
-      float s_next = k0 < k1 ? __ldg(sa + (int64_t)k0 * g.M) * __ldg(sb + k0) : 0.f;
-      for (int kb = k0; kb < k1; ++kb, ++it) {
+      for (int i = 0; i < kCols / 32; ++i) {
+        const int c = col0 + 32 * i + lane;
+        bias_next[i] = (g.bias != nullptr && c < g.N) ? __ldg(g.bias + c) : 0.f;
+      }
+    };
+    uint32_t tile = blockIdx.x;
+    Place p = place(tile);
+    if (tile < g.tiles) aim(p);
+    while (tile < g.tiles) {
+      const int64_t row0 = (int64_t)p.mt * kTileM + quarter * 32;
+      const int col0 = p.nt * kTileN + part * kCols;
+      const int sp = p.sp, blocks = p.k1 - p.k0;
+      tile += gridDim.x;
+      if (tile < g.tiles) p = place(tile);
+      __syncwarp();  // the previous tile's bias has been read
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) bias_s[32 * i + lane] = bias_next[i];
+      __syncwarp();
+      float acc[kCols];  // starts as the bias
+#pragma unroll
+      for (int i = 0; i < kCols / 4; ++i) {
+        const float4 v = reinterpret_cast<const float4 *>(bias_s)[i];
+        acc[4 * i] = v.x; acc[4 * i + 1] = v.y; acc[4 * i + 2] = v.z; acc[4 * i + 3] = v.w;
+      }
+      for (int kb = 0; kb < blocks; ++kb, ++it) {
         const int buf = it % B;
-        const float s = s_next;
-        if (kb + 1 < k1) s_next = __ldg(sa + (int64_t)(kb + 1) * g.M) * __ldg(sb + kb + 1);
+        const float sa_now = sa_next, sb_now = sb_next;
+        if (kb + 1 < blocks) {
+          sa += g.M;
+          ++sb;
+          sa_next = __ldg(sa);
+          sb_next = __ldg(sb);
+        } else if (tile < g.tiles) {
+          aim(p);
+        }
         dead = !__all_sync(kFull, mbar_wait(&sh.acc_full[buf], (it / B) & 1, &sh.abort));
         if (dead) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kTileN + part * 64);
+        float s;  // volatile: stays behind the wait.  Left to the compiler the product moved up to where its
+                  // factors are loaded, and every block waited for that load: 460 of 1200 cycles
+        asm volatile("mul.f32 %0, %1, %2;" : "=f"(s) : "f"(sa_now), "f"(sb_now));
+        const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kTileN + part * kCols);
         uint32_t r[2][16];
         tmem_load_16_issue(taddr, r[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kCols / 16; ++c) {
           tmem_load_16_wait(r[c & 1]);
-          if (c < 3) {
+          if (c + 1 < kCols / 16) {
             tmem_load_16_issue(taddr + 16 * (c + 1), r[(c + 1) & 1]);
           } else {  // the last read has landed: the accumulator goes back
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(&sh.acc_empty[buf]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.acc_empty[buf]);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(s, __uint_as_float(r[c & 1][i]), acc[16 * c + i]);
         }
       }
       if (dead) break;
-      __syncwarp();
-      {
-        const float4 *b = reinterpret_cast<const float4 *>(sh.bias[warp - 2]);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float4 v = b[i];
-          acc[4 * i] += v.x; acc[4 * i + 1] += v.y; acc[4 * i + 2] += v.z; acc[4 * i + 3] += v.w;
-        }
-      }
-      // rows leave through the warp's staging tile, 64 bytes of each at a time
-      constexpr int kChunk = 64 / (int)sizeof(OutT);
+      // rows leave through the warp's staging tiles, 128 bytes of each in one tile
+      constexpr int kChunk = 128 / (int)sizeof(OutT);
+      constexpr int kChunks = kCols / kChunk;
       const int rows_here = (int)min((int64_t)32, g.M - row0);
-      unsigned char *out = g.out + ((int64_t)sp * g.M + row0) * g.N * (int64_t)sizeof(OutT) + (int64_t)col0 * sizeof(OutT);
       const int64_t pitch = (int64_t)g.N * sizeof(OutT);
+      unsigned char *out = g.out + ((int64_t)sp * g.out_rows + row0) * pitch + (int64_t)col0 * sizeof(OutT);
 #pragma unroll
-      for (int c = 0; c < 64 / kChunk; ++c) {
-        const int bytes = min(64, (g.N - col0) * (int)sizeof(OutT) - c * 64);
-        if (bytes <= 0 || rows_here <= 0) break;  // warp-uniform
-        uint4 *mine = reinterpret_cast<uint4 *>(staged + lane * kStagePitch);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 w;
-          if constexpr (sizeof(OutT) == 4) {
-            w = make_uint4(__float_as_uint(acc[16 * c + 4 * i]), __float_as_uint(acc[16 * c + 4 * i + 1]),
-                           __float_as_uint(acc[16 * c + 4 * i + 2]), __float_as_uint(acc[16 * c + 4 * i + 3]));
-          } else {
-            const float *p = acc + 32 * c + 8 * i;
-            w = make_uint4(pack_pair<OutT>(p[0], p[1]), pack_pair<OutT>(p[2], p[3]), pack_pair<OutT>(p[4], p[5]), pack_pair<OutT>(p[6], p[7]));
-          }
-          mine[i] = w;
+      for (int c0 = 0; c0 < kChunks; c0 += S::staged_tiles) {
+        if (rows_here <= 0) break;
+        if (g.unit == 0) {  // the stores that used the tiles have read them
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
         }
+#pragma unroll
+        for (int k = 0; k < S::staged_tiles && c0 + k < kChunks; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint4 w;
+            if constexpr (sizeof(OutT) == 4) {
+              const float *v = acc + 32 * (c0 + k) + 4 * i;
+              w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            } else {
+              const float *v = acc + 64 * (c0 + k) + 8 * i;
+              w = make_uint4(round_pair<OutT>(v[0], v[1]), round_pair<OutT>(v[2], v[3]), round_pair<OutT>(v[4], v[5]), round_pair<OutT>(v[6], v[7]));
+            }
+            *reinterpret_cast<uint4 *>(staging_tiles + k * kStagedBytes + staged_at(lane, i)) = w;
+          }
+        if (g.unit == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (g.unit == 16) store_staged<uint4>(staged, out + c * 64, pitch, rows_here, bytes, lane);
-        else if (g.unit == 8) store_staged<uint2>(staged, out + c * 64, pitch, rows_here, bytes, lane);
-        else if (g.unit == 4) store_staged<uint32_t>(staged, out + c * 64, pitch, rows_here, bytes, lane);
-        else store_staged<uint16_t>(staged, out + c * 64, pitch, rows_here, bytes, lane);
-        __syncwarp();
+        if (g.unit == 0) {
+          // what lies beyond the matrix is not written
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < S::staged_tiles && c0 + k < kChunks; ++k)
+              if (col0 + (c0 + k) * kChunk < g.N)
+                tma_store_2d(&map_out, staging_tiles + k * kStagedBytes, col0 + (c0 + k) * kChunk, (int)(sp * g.out_rows + row0));
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < S::staged_tiles && c0 + k < kChunks; ++k) {
+            const unsigned char *staged = staging_tiles + k * kStagedBytes;
+            unsigned char *dst = out + (c0 + k) * 128;
+            const int bytes = min(128, (g.N - col0) * (int)sizeof(OutT) - (c0 + k) * 128);
+            if (bytes <= 0) break;  // warp-uniform
+            if (g.unit == 8) store_staged<uint2>(staged, dst, pitch, rows_here, bytes, lane);
+            else if (g.unit == 4) store_staged<uint32_t>(staged, dst, pitch, rows_here, bytes, lane);
+            else store_staged<uint16_t>(staged, dst, pitch, rows_here, bytes, lane);
+          }
+          __syncwarp();
+        }
       }
     }
+    if (g.unit == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -530,12 +599,12 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // out = sum over the pieces of K (in their order) + bias, rounded once.
 template <typename OutT>
 __global__ void __launch_bounds__(256)
-split_sum_kernel(const float *__restrict__ part, int splits, int64_t count, int N, const float *__restrict__ bias, OutT *__restrict__ out) {
+split_sum_kernel(const float *__restrict__ part, int splits, int64_t stride, int64_t count, int N, const float *__restrict__ bias, OutT *__restrict__ out) {
   pdl_wait();
   pdl_trigger();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
     float sum = bias != nullptr ? __ldg(bias + i % N) : 0.f;
-    for (int s = 0; s < splits; ++s) sum += __ldg(part + (int64_t)s * count + i);
+    for (int s = 0; s < splits; ++s) sum += __ldg(part + (int64_t)s * stride + i);
     out[i] = (OutT)sum;
   }
 }
@@ -560,28 +629,31 @@ MatmulPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
   return {tile_n, splits};
 }
 
+// Rows of one piece's partial sums: whole row tiles, so that a store never reaches the next piece's.
+int64_t whole_tiles(int64_t M) { return (M + kTileM - 1) / kTileM * kTileM; }
+
 template <int kTileN, typename OutT>
-cudaError_t launch_matmul(const CUtensorMap &ma, const CUtensorMap &mb, MatmulArgs g, cudaStream_t s) {
+cudaError_t launch_matmul(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const MatmulArgs &g, cudaStream_t s) {
   static SmemGrant grant;
   const cudaError_t e = grant.ensure(fp8_matmul_kernel<kTileN, OutT>, Shape<kTileN>::smem);
   if (e != cudaSuccess) return e;
   const int sms = sm_count();
-  const unsigned grid = (unsigned)(g.tiles < sms ? g.tiles : sms);
-  return launch_pdl(fp8_matmul_kernel<kTileN, OutT>, grid, (unsigned)Shape<kTileN>::threads, Shape<kTileN>::smem, s, ma, mb, g);
+  const unsigned grid = g.tiles < (unsigned)sms ? g.tiles : (unsigned)sms;
+  return launch_pdl(fp8_matmul_kernel<kTileN, OutT>, grid, (unsigned)Shape<kTileN>::threads, Shape<kTileN>::smem, s, ma, mb, mo, g);
 }
 
 template <typename OutT>
-cudaError_t launch_matmul_n(int tile_n, const CUtensorMap &ma, const CUtensorMap &mb, const MatmulArgs &g, cudaStream_t s) {
-  if (tile_n == 256) return launch_matmul<256, OutT>(ma, mb, g, s);
-  if (tile_n == 128) return launch_matmul<128, OutT>(ma, mb, g, s);
-  return launch_matmul<64, OutT>(ma, mb, g, s);
+cudaError_t launch_matmul_n(int tile_n, const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const MatmulArgs &g, cudaStream_t s) {
+  if (tile_n == 256) return launch_matmul<256, OutT>(ma, mb, mo, g, s);
+  if (tile_n == 128) return launch_matmul<128, OutT>(ma, mb, mo, g, s);
+  return launch_matmul<64, OutT>(ma, mb, mo, g, s);
 }
 
 template <typename OutT>
-cudaError_t launch_split_sum(const float *part, int splits, int64_t count, int N, const float *bias, void *out, cudaStream_t s) {
+cudaError_t launch_split_sum(const float *part, int splits, int64_t stride, int64_t count, int N, const float *bias, void *out, cudaStream_t s) {
   const int64_t blocks = (count + 255) / 256;
   return launch_pdl(split_sum_kernel<OutT>, (unsigned)std::min<int64_t>(blocks, 16 * (int64_t)sm_count()), 256u, 0, s,
-                    part, splits, count, N, bias, static_cast<OutT *>(out));
+                    part, splits, stride, count, N, bias, static_cast<OutT *>(out));
 }
 
 template <typename T>
@@ -638,7 +710,7 @@ int ot_b200_fp8_quantize(const void *d_x, int64_t rows, int32_t cols, int64_t ro
   if (a.row_tiles * a.col_tiles > INT32_MAX)
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: more than 2^31 - 1 blocks of 128 x 128");
   const size_t es = types ? 2 : 4;
-  a.vec = reinterpret_cast<uintptr_t>(d_x) % (4 * es) == 0 && row_stride % 4 == 0;
+  a.vec = reinterpret_cast<uintptr_t>(d_x) % (4 * es) == 0 && row_stride % 4 == 0 && cols % 4 == 0;
   a.q = static_cast<uint8_t *>(d_q);
   a.q_pitch = q_pitch;
   a.scale = d_scale;
@@ -663,7 +735,7 @@ int ot_b200_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, uint64_t
   if (!bytes_out || M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: sizes must be 1..2^31-1");
   const MatmulPlan p = plan_matmul(M, N, K, sm_count());
-  *bytes_out = p.splits > 1 ? (uint64_t)p.splits * M * N * sizeof(float) : 0;
+  *bytes_out = p.splits > 1 ? (uint64_t)p.splits * whole_tiles(M) * N * sizeof(float) : 0;
   return OT_B200_OK;
 }
 
@@ -700,22 +772,33 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
   g.k_blocks = (int)((K + kScaleBlock - 1) / kScaleBlock);
   g.n_tiles = (int)((N + p.tile_n - 1) / p.tile_n);
   g.splits = p.splits;
-  g.tiles = (M + kTileM - 1) / kTileM * g.n_tiles * p.splits;
+  const int64_t tiles = (M + kTileM - 1) / kTileM * g.n_tiles * p.splits;
+  if (tiles > INT32_MAX) return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: more than 2^31 - 1 tiles");
+  g.tiles = (uint32_t)tiles;
   const bool split = p.splits > 1;
   g.bias = split ? nullptr : d_bias;
   g.out = static_cast<unsigned char *>(split ? d_workspace : d_out);
-  const uint64_t where = reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(N * (split ? sizeof(float) : es));
-  g.unit = where % 16 == 0 ? 16 : (where % 8 == 0 ? 8 : (where % 4 == 0 ? 4 : 2));
+  g.out_rows = split ? whole_tiles(M) : M;
+  const size_t out_es = split ? sizeof(float) : es;
+  const uint64_t where = reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(N * out_es);
+  g.unit = where % 16 == 0 ? 0 : (where % 8 == 0 ? 8 : (where % 4 == 0 ? 4 : 2));
+  CUtensorMap mo;
+  memset(&mo, 0, sizeof(mo));
+  // (stores in float are split over 32 columns, in 16 bits over 64: 128 bytes)
+  if (g.unit == 0 &&
+      !make_tensor_map(&mo, out_es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, g.out,
+                       (uint64_t)(p.splits * g.out_rows), (uint64_t)N, (uint64_t)(N * out_es), 32, (uint32_t)(128 / out_es)))
+    g.unit = 8;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (split || types == 0) e = launch_matmul_n<float>(p.tile_n, ma, mb, g, s);
-  else if (types == OT_B200_BF16) e = launch_matmul_n<__nv_bfloat16>(p.tile_n, ma, mb, g, s);
-  else e = launch_matmul_n<__half>(p.tile_n, ma, mb, g, s);
+  if (split || types == 0) e = launch_matmul_n<float>(p.tile_n, ma, mb, mo, g, s);
+  else if (types == OT_B200_BF16) e = launch_matmul_n<__nv_bfloat16>(p.tile_n, ma, mb, mo, g, s);
+  else e = launch_matmul_n<__half>(p.tile_n, ma, mb, mo, g, s);
   if (e == cudaSuccess && split) {
     const float *part = static_cast<const float *>(d_workspace);
-    if (types == 0) e = launch_split_sum<float>(part, p.splits, M * N, (int)N, d_bias, d_out, s);
-    else if (types == OT_B200_BF16) e = launch_split_sum<__nv_bfloat16>(part, p.splits, M * N, (int)N, d_bias, d_out, s);
-    else e = launch_split_sum<__half>(part, p.splits, M * N, (int)N, d_bias, d_out, s);
+    if (types == 0) e = launch_split_sum<float>(part, p.splits, g.out_rows * N, M * N, (int)N, d_bias, d_out, s);
+    else if (types == OT_B200_BF16) e = launch_split_sum<__nv_bfloat16>(part, p.splits, g.out_rows * N, M * N, (int)N, d_bias, d_out, s);
+    else e = launch_split_sum<__half>(part, p.splits, g.out_rows * N, M * N, (int)N, d_bias, d_out, s);
   }
   if (e != cudaSuccess) return fail(OT_B200_ERR_CUDA, "ot_b200_fp8_matmul: %s", cudaGetErrorString(e));
   return OT_B200_OK;

@@ -387,17 +387,21 @@ template <typename T> __device__ __forceinline__ float to_float(T x) { return (f
 template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]);
-template <> __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
-  const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+// The load and the conversion are apart, so that a kernel can request all its loads
+// before the first is used.
+template <typename T> struct Raw4 { typedef uint2 type; };
+template <> struct Raw4<float> { typedef float4 type; };
+template <typename T> __device__ __forceinline__ typename Raw4<T>::type load4(const T *p) {
+  return __ldg(reinterpret_cast<const typename Raw4<T>::type *>(p));
 }
-template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]) {
-  const uint2 a = __ldg(reinterpret_cast<const uint2 *>(p));
+template <typename T> __device__ __forceinline__ void convert4(const uint2 &raw, float (&v)[4]) {
   T t[4];
-  memcpy(t, &a, sizeof(a));
+  memcpy(t, &raw, sizeof(raw));
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = to_float(t[i]);
+}
+template <typename T> __device__ __forceinline__ void convert4(const float4 &raw, float (&v)[4]) {
+  v[0] = raw.x; v[1] = raw.y; v[2] = raw.z; v[3] = raw.w;
 }
 
 template <typename T> __device__ __forceinline__ T neg_inf();

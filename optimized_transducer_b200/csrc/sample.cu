@@ -45,7 +45,7 @@ struct SampleArgs {
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
   float eps;
-  bool vec;              // four logits may be loaded at once
+  bool vec;              // four logits may be loaded at once, and V is a multiple of four
   int32_t *token;
   float *logprob;
 };
@@ -298,17 +298,27 @@ sample_kernel(const SampleArgs a) {
 
   float x[E];
   const T *src = static_cast<const T *>(a.logits) + row * a.stride;
+  if (a.vec) {
+    // groups of four lie inside the row or outside; all loads are requested before one is used
+    typename Raw4<T>::type raw[J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int at = first + 4 * (j * kWarps * 32 + tid);
-    if (a.vec && at + 3 < a.V) {
+    for (int j = 0; j < J; ++j) {
+      const int at = first + 4 * (j * kWarps * 32 + tid);
+      raw[j] = typename Raw4<T>::type{};
+      if (at < a.V) raw[j] = load4(src + at);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
       float f[4];
-      load4<T>(src + at, f);
+      convert4<T>(raw[j], f);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x[4 * j + q] = f[q];
-    } else {
+      for (int q = 0; q < 4; ++q) x[4 * j + q] = first + 4 * (j * kWarps * 32 + tid) < a.V ? f[q] : -inf_f();
+    }
+  } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x[4 * j + q] = at + q < a.V ? to_float(src[at + q]) : -inf_f();
+    for (int e = 0; e < E; ++e) {
+      const int at = first + 4 * ((e >> 2) * kWarps * 32 + tid) + (e & 3);
+      x[e] = at < a.V ? to_float(__ldg(src + at)) : -inf_f();
     }
   }
   const float u = __ldg(a.u + row);
@@ -581,7 +591,7 @@ extern "C" int ot_b200_sample(const void *d_logits, int64_t rows, int32_t V, int
   a.min_p_all = min_p;
   a.top_k_all = top_k;
   const size_t es = types ? 2 : 4;
-  a.vec = reinterpret_cast<uintptr_t>(d_logits) % (4 * es) == 0 && (rows == 1 || row_stride % 4 == 0);
+  a.vec = reinterpret_cast<uintptr_t>(d_logits) % (4 * es) == 0 && (rows == 1 || row_stride % 4 == 0) && V % 4 == 0;
   a.token = d_tokens;
   a.logprob = d_logprobs;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
