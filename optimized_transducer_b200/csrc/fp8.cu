@@ -85,67 +85,105 @@ struct QuantArgs {
   float *column_sums;   // [row tile][column], or NULL
 };
 
+// A lane's four elements of one row as they were loaded.
+template <typename T> struct Quad {
+  typename Raw4<T>::type raw;
+  __device__ __forceinline__ void clear() { raw = typename Raw4<T>::type{}; }
+  __device__ __forceinline__ void set(int j, T x) {
+    T t[4];
+    memcpy(t, &raw, sizeof(raw));
+    t[j] = x;
+    memcpy(&raw, t, sizeof(raw));
+  }
+  __device__ __forceinline__ float at(int j) const {
+    T t[4];
+    memcpy(t, &raw, sizeof(raw));
+    return to_float(t[j]);
+  }
+  // Bits of |x| of the four, of the largest; bits of |x| order as unsigned integers do, also
+  // those of the 16-bit types, so two of these are compared at a time.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 4) {
+      return max(max(abs_bits(at(0)), abs_bits(at(1))), max(abs_bits(at(2)), abs_bits(at(3))));
+    } else {
+      uint32_t w[2];
+      memcpy(w, &raw, 8);
+      const uint32_t m = __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
+      return widen(max(m & 0xffffu, m >> 16));
+    }
+  }
+  // Float bits of |x| from the bits of the element type's |x|.
+  __device__ __forceinline__ static uint32_t widen(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) {
+      return bits;
+    } else {
+      const uint16_t b = (uint16_t)bits;
+      T t;
+      memcpy(&t, &b, 2);
+      return __float_as_uint(to_float(t));
+    }
+  }
+};
+
 // One block per 128 x 128 tile of x; a warp holds 16 rows, a lane four columns of each, in
-// registers, so the tile is read once whatever is written: bytes along the rows (kPlain),
-// transposed bytes (kTrans), and the tile's column sums.  Bound by HBM: sizeof(T) bytes
-// read and one or two written per element.
+// registers and in the type they have (half the registers in 16 bits: three blocks per SM
+// instead of one), so the tile is read once whatever is written: bytes along the rows
+// (kPlain), transposed bytes (kTrans), and the tile's column sums.  Bound by HBM: sizeof(T)
+// bytes read and one or two written per element.
 template <typename T, int kPlain, int kTrans, bool kSums>
-__global__ void __launch_bounds__(kQuantThreads)
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 3 : 2)
 quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
   __shared__ uint32_t top_s[8][kScaleBlock];   // column maxima of each warp (or one word per warp)
   __shared__ float sum_s[kSums ? 8 : 1][kScaleBlock];
   __shared__ float inv_s[kScaleBlock];
   __shared__ __align__(16) uint8_t tile_s[kTrans != kNone ? kScaleBlock * kScaleBlock : 16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t rt = blockIdx.x / a.col_tiles;
-  const int ct = (int)(blockIdx.x - rt * a.col_tiles);
-  const int64_t row0 = rt * kScaleBlock + warp * kQuantRows;
+  const uint32_t rt = blockIdx.x / (uint32_t)a.col_tiles;
+  const int ct = (int)(blockIdx.x - rt * (uint32_t)a.col_tiles);
+  const int64_t row0 = (int64_t)rt * kScaleBlock + warp * kQuantRows;
   const int col0 = ct * kScaleBlock, col = col0 + 4 * lane;
+  const int rows_here = (int)min((int64_t)kQuantRows, max((int64_t)0, a.rows - row0));
   pdl_wait();
   pdl_trigger();
 
-  float v[kQuantRows][4];
+  Quad<T> v[kQuantRows];
+  const T *p = x + row0 * a.ld + col;
   if (a.vec) {
     // groups of four lie inside a row or outside; all loads are requested before one is used
-    typename Raw4<T>::type raw[kQuantRows];
-    const T *p = x + row0 * a.ld + col;
 #pragma unroll
     for (int i = 0; i < kQuantRows; ++i) {
-      raw[i] = typename Raw4<T>::type{};
-      if (row0 + i < a.rows && col < a.cols) raw[i] = load4(p + i * a.ld);
+      v[i].clear();
+      if (i < rows_here && col < a.cols) v[i].raw = load4(p + i * a.ld);
     }
-#pragma unroll
-    for (int i = 0; i < kQuantRows; ++i) convert4<T>(raw[i], v[i]);
   } else {
-    const T *p = x + row0 * a.ld + col;
 #pragma unroll
-    for (int i = 0; i < kQuantRows; ++i)
+    for (int i = 0; i < kQuantRows; ++i) {
+      v[i].clear();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = row0 + i < a.rows && col + j < a.cols ? to_float(__ldg(p + i * a.ld + j)) : 0.f;
+      for (int j = 0; j < 4; ++j)
+        if (i < rows_here && col + j < a.cols) v[i].set(j, p[i * a.ld + j]);
+    }
   }
 
   if constexpr (kPlain == kRowBlocks) {
     float mine = 0.f;
+    uint8_t *q = a.q + row0 * a.q_pitch + col;
 #pragma unroll
     for (int i = 0; i < kQuantRows; ++i) {
-      uint32_t top = max(max(abs_bits(v[i][0]), abs_bits(v[i][1])), max(abs_bits(v[i][2]), abs_bits(v[i][3])));
-      top = __reduce_max_sync(kFull, top);
+      const uint32_t top = __reduce_max_sync(kFull, v[i].top());
       float inv;
       const float s = block_scale(top, inv);
       if (lane == i) mine = s;
-      if (row0 + i < a.rows && col < a.cols)  // the pitch is a multiple of 16: the word stays inside the row
-        *reinterpret_cast<uint32_t *>(a.q + (row0 + i) * a.q_pitch + col) =
-            pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+      if (i < rows_here && col < a.cols)  // the pitch is a multiple of 16: the word stays inside the row
+        *reinterpret_cast<uint32_t *>(q + i * a.q_pitch) = pack4(v[i].at(0) * inv, v[i].at(1) * inv, v[i].at(2) * inv, v[i].at(3) * inv);
     }
-    if (lane < kQuantRows && row0 + lane < a.rows) a.scale[(int64_t)ct * a.rows + row0 + lane] = mine;
+    if (lane < rows_here) a.scale[(int64_t)ct * a.rows + row0 + lane] = mine;
   }
   float square_inv = 0.f;
   if constexpr (kPlain == kSquareBlocks || kTrans == kSquareBlocks) {
     uint32_t top = 0u;
 #pragma unroll
-    for (int i = 0; i < kQuantRows; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = max(top, abs_bits(v[i][j]));
+    for (int i = 0; i < kQuantRows; ++i) top = max(top, v[i].top());
     top = __reduce_max_sync(kFull, top);
     if (lane == 0) top_s[0][warp] = top;
     __syncthreads();
@@ -154,15 +192,16 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
     for (int w = 0; w < 8; ++w) top = max(top, top_s[0][w]);
     const float s = block_scale(top, square_inv);
     if (threadIdx.x == 0) {
-      if (kPlain == kSquareBlocks) a.scale[rt * a.col_tiles + ct] = s;
+      if (kPlain == kSquareBlocks) a.scale[(int64_t)rt * a.col_tiles + ct] = s;
       if (kTrans == kSquareBlocks) a.scale_t[(int64_t)ct * a.row_tiles + rt] = s;
     }
     if (kPlain == kSquareBlocks) {
+      uint8_t *q = a.q + row0 * a.q_pitch + col;
 #pragma unroll
       for (int i = 0; i < kQuantRows; ++i)
-        if (row0 + i < a.rows && col < a.cols)
-          *reinterpret_cast<uint32_t *>(a.q + (row0 + i) * a.q_pitch + col) =
-              pack4(v[i][0] * square_inv, v[i][1] * square_inv, v[i][2] * square_inv, v[i][3] * square_inv);
+        if (i < rows_here && col < a.cols)
+          *reinterpret_cast<uint32_t *>(q + i * a.q_pitch) =
+              pack4(v[i].at(0) * square_inv, v[i].at(1) * square_inv, v[i].at(2) * square_inv, v[i].at(3) * square_inv);
     }
   }
   if constexpr (kTrans == kColumnBlocks || kSums) {
@@ -172,8 +211,9 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kQuantRows; ++i) {
-        top = max(top, abs_bits(v[i][j]));
-        sum += v[i][j];
+        const float f = v[i].at(j);
+        top = max(top, abs_bits(f));
+        sum += f;
       }
       if (kTrans == kColumnBlocks) top_s[warp][4 * lane + j] = top;
       if (kSums) sum_s[warp][4 * lane + j] = sum;
@@ -188,13 +228,13 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
         float inv;
         const float s = block_scale(top, inv);
         inv_s[c] = inv;
-        if (col0 + c < a.cols) a.scale_t[rt * a.cols + col0 + c] = s;
+        if (col0 + c < a.cols) a.scale_t[(int64_t)rt * a.cols + col0 + c] = s;
       }
       if (kSums) {
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) sum += sum_s[w][c];
-        if (col0 + c < a.cols) a.column_sums[rt * a.cols + col0 + c] = sum;
+        if (col0 + c < a.cols) a.column_sums[(int64_t)rt * a.cols + col0 + c] = sum;
       }
     }
     __syncthreads();
@@ -206,18 +246,17 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float inv = kTrans == kSquareBlocks ? square_inv : inv_s[4 * lane + j];
-      uint4 w;
-      w.x = pack4(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
-      w.y = pack4(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv);
-      w.z = pack4(v[8][j] * inv, v[9][j] * inv, v[10][j] * inv, v[11][j] * inv);
-      w.w = pack4(v[12][j] * inv, v[13][j] * inv, v[14][j] * inv, v[15][j] * inv);
-      *reinterpret_cast<uint4 *>(tile_s + (4 * lane + j) * kScaleBlock + 16 * (warp ^ (lane & 7))) = w;
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = pack4(v[4 * k].at(j) * inv, v[4 * k + 1].at(j) * inv, v[4 * k + 2].at(j) * inv, v[4 * k + 3].at(j) * inv);
+      *reinterpret_cast<uint4 *>(tile_s + (4 * lane + j) * kScaleBlock + 16 * (warp ^ (lane & 7))) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncthreads();
 #pragma unroll
     for (int i = threadIdx.x; i < kScaleBlock * 8; i += kQuantThreads) {
       const int c = i >> 3, piece = i & 7;
-      const int64_t at = rt * kScaleBlock + 16 * piece;
+      const int64_t at = (int64_t)rt * kScaleBlock + 16 * piece;
       if (col0 + c < a.cols && at < a.qt_pitch)
         *reinterpret_cast<uint4 *>(a.qt + (int64_t)(col0 + c) * a.qt_pitch + at) =
             *reinterpret_cast<const uint4 *>(tile_s + c * kScaleBlock + 16 * (piece ^ ((c >> 2) & 7)));
