@@ -12,19 +12,24 @@
 // no counterpart: decoding lies outside its loss.
 //
 // Whole numbers have to come out right, so the answer is DEFINED in 64 bits.  The work is
-// done in float: with E logits per thread the float sum of any subset of the w is off by
-// at most
-//     eps * (sum of w),   eps = (3 ln V + E + 24) * 2^-24
-// (3 * 2^-24 per unit of the exponent's argument from the subtraction, the factor and the
-// product, and sum w_i |ln w_i| <= ln V * sum w_i; 2^-22 from ex2.approx; one rounding per
-// addition on the longest path), and a comparison of two such sums that is closer than
-// twice that is made again with double sums.  Nothing is sorted: a filter's border is a
-// logit, found by bisection between the logits that are still in question.
+// done in float: the float sum of any subset of the w is off by at most
+//     eps * (sum of w)
+// where a row of up to 1024 has eps = (3 ln V + n + 6) * 2^-24: 2^-24 per unit of the
+// exponent's argument from the subtraction, the factor and the product, sum w_i |ln w_i|
+// <= ln V * sum w_i, ex2.approx is good to 2^-22, and n additions lie on the longest path.
+// In wider rows more sums come close to each other: there the argument is carried in two
+// floats and sums of four weights are added in double, so eps = 9 * 2^-24.  A
+// comparison of two such sums that is closer than twice that is made again with double sums
+// (about one row in a hundred at 500 symbols).  Nothing is sorted: a filter's border is a
+// logit, found by bisection on the values and then between the logits that are still in
+// question.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "ot_common.cuh"
 
@@ -44,7 +49,7 @@ struct SampleArgs {
   const int32_t *top_k;
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
-  float eps;
+  float eps, eps_steps;
   bool vec;              // four logits may be loaded at once, and V is a multiple of four
   int32_t *token;
   float *logprob;
@@ -76,9 +81,16 @@ template <typename A> struct Pass {
 // cluster.  Reductions and searches give every thread the same answer, in a fixed order of
 // additions.  The scratch is used in two halves in turn, so one barrier per reduction will do.
 template <int kWarps, int kCtas> struct Team {
+  using Sum = typename std::conditional<kWarps == 1, float, double>::type;
+  static_assert(kCtas <= kWarps, "a warp hands sums to each block");
+  // Logits that one step of a search compares with.  One inside a block, where instructions
+  // are the bound (eight: 10 700 instructions per warp and row of 5000 against 3 000); four
+  // across blocks, where a step waits for the cluster's barrier: 2.3 bits of the border per step.
+  static constexpr int kPivots = kCtas == 1 ? 1 : 4;
   struct Scratch {
     Pass<double> warp_part[2][kWarps];
     Pass<double> cta_part[2][kCtas];
+    float warp_sums[2][kWarps][kPivots], cta_sums[2][kCtas][kPivots];
     double table[16][kWarps];
     int index;
     double before, upto;
@@ -89,50 +101,94 @@ template <int kWarps, int kCtas> struct Team {
   __device__ explicit Team(Scratch &scratch) : s(scratch) {}
 
   // kWhat: which fields are asked for (kSum, kCount, kEnds); the others come back unreduced.
-  template <int kWhat, typename A> __device__ __forceinline__ Pass<A> reduce(Pass<A> p) {
+  template <int kWhat, typename A> __device__ __forceinline__ static Pass<A> across(Pass<A> p) {
     if (kWhat & kSum) p.sum = warp_sum(p.sum);
     if (kWhat & kCount) p.count = __reduce_add_sync(kFull, p.count);
     if (kWhat & kEnds) {
       p.least = warp_min_f(p.least);
       p.most = warp_max_f(p.most);
     }
+    return p;
+  }
+  template <typename A, int kN> __device__ __forceinline__ static Pass<A> entry(const Pass<double> (&part)[kN]) {
+    const int lane = threadIdx.x & 31;
+    if (lane >= kN) return Pass<A>{A(0), 0, inf_f(), -inf_f()};
+    const Pass<double> &t = part[lane];
+    return Pass<A>{(A)t.sum, t.count, t.least, t.most};
+  }
+  template <int kWhat, typename A> __device__ __forceinline__ Pass<A> reduce(Pass<A> p) {
+    p = across<kWhat>(p);
     if constexpr (kWarps > 1) {
-      const int warp = threadIdx.x >> 5;
       half ^= 1;
-      if ((threadIdx.x & 31) == 0) s.warp_part[half][warp] = Pass<double>{(double)p.sum, p.count, p.least, p.most};
+      if ((threadIdx.x & 31) == 0) s.warp_part[half][threadIdx.x >> 5] = Pass<double>{(double)p.sum, p.count, p.least, p.most};
       __syncthreads();
-      Pass<double> t = s.warp_part[half][0];
-      A sum = (A)t.sum;
-#pragma unroll 8
-      for (int w = 1; w < kWarps; ++w) {
-        const Pass<double> o = s.warp_part[half][w];
-        sum += (A)o.sum;
-        t.count += o.count;
-        t.least = fminf(t.least, o.least);
-        t.most = fmaxf(t.most, o.most);
-      }
-      p = Pass<A>{sum, t.count, t.least, t.most};
+      p = across<kWhat>(entry<A>(s.warp_part[half]));
     }
     if constexpr (kCtas > 1) {
       cg::cluster_group cluster = cg::this_cluster();
-      if (threadIdx.x < kCtas) {
-        Pass<double> *there = cluster.map_shared_rank(&s.cta_part[half][cluster.block_rank()], threadIdx.x);
-        *there = Pass<double>{(double)p.sum, p.count, p.least, p.most};
-      }
+      if (threadIdx.x < kCtas)
+        *cluster.map_shared_rank(&s.cta_part[half][cluster.block_rank()], threadIdx.x) = Pass<double>{(double)p.sum, p.count, p.least, p.most};
       cluster.sync();
-      Pass<double> t = s.cta_part[half][0];
-      A sum = (A)t.sum;
-#pragma unroll
-      for (int c = 1; c < kCtas; ++c) {
-        const Pass<double> o = s.cta_part[half][c];
-        sum += (A)o.sum;
-        t.count += o.count;
-        t.least = fminf(t.least, o.least);
-        t.most = fmaxf(t.most, o.most);
-      }
-      p = Pass<A>{sum, t.count, t.least, t.most};
+      p = across<kWhat>(entry<A>(s.cta_part[half]));
     }
     return p;
+  }
+
+  __device__ __forceinline__ float max_with_nan(float v) {
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(v) : "f"(v));
+    if constexpr (kWarps > 1) {  // as a count and a maximum: the reduction of several warps drops a NaN
+      const Pass<float> p = reduce<kCount | kEnds>(Pass<float>{0.f, v != v ? 1 : 0, 0.f, v});
+      return p.count ? __int_as_float(0x7fffffff) : p.most;
+    }
+    return v;
+  }
+
+  // Sums of kPivots values at once: a lane gets the sum of the value mine() names.  Each of
+  // the first steps hands half of the values to the neighbour, so the sums of four
+  // values take six exchanges and not twenty.
+  __device__ __forceinline__ static int mine(int lane) {
+    return kPivots == 4 ? ((lane & 1) << 1 | (lane & 2) >> 1) : 0;
+  }
+  __device__ __forceinline__ float sum_each(float (&v)[kPivots]) {
+    const int lane = threadIdx.x & 31;
+    int bit = 1;
+#pragma unroll
+    for (int n = kPivots; n > 1; n >>= 1, bit <<= 1) {
+      const bool upper = (lane & bit) != 0;
+#pragma unroll
+      for (int i = 0; i < n / 2; ++i) {
+        const float give = upper ? v[i] : v[i + n / 2];
+        v[i] = (upper ? v[i + n / 2] : v[i]) + __shfl_xor_sync(kFull, give, bit);
+      }
+    }
+    float t = v[0];
+#pragma unroll
+    for (int o = kPivots; o < 32; o <<= 1) t += __shfl_xor_sync(kFull, t, o);
+    if constexpr (kWarps > 1) {
+      half ^= 1;
+      if (lane < kPivots) s.warp_sums[half][threadIdx.x >> 5][lane] = t;
+      __syncthreads();
+      t = gather(s.warp_sums[half]);
+    }
+    if constexpr (kCtas > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      // the first kPivots lanes of warp c hand the block's sums to block c
+      if ((threadIdx.x >> 5) < kCtas && lane < kPivots)
+        cluster.map_shared_rank(&s.cta_sums[half][cluster.block_rank()][0], threadIdx.x >> 5)[lane] = t;
+      cluster.sync();
+      t = gather(s.cta_sums[half]);
+    }
+    return t;
+  }
+  template <int kN> __device__ __forceinline__ static float gather(const float (&part)[kN][kPivots]) {
+    const int lane = threadIdx.x & 31;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kN; w += 32 / kPivots)
+      if (w + lane / kPivots < kN) t += part[w + lane / kPivots][lane % kPivots];
+#pragma unroll
+    for (int o = kPivots; o < 32; o <<= 1) t += __shfl_xor_sync(kFull, t, o);
+    return t;
   }
 
   // The first element, in index order, at which the running sum of value(x, w) exceeds
@@ -140,16 +196,31 @@ template <int kWarps, int kCtas> struct Team {
   // Element e = 4 j + q of thread t has the index first + 4 (j * threads + t) + q.
   template <typename A> struct Found { int index; A before, upto; };
 
-  template <int J, typename A, typename F>
+  // kRolled: value() is costly and few rows ask for it, so the loop is not unrolled, and
+  // `target` is a fraction of the sum of all values.
+  template <int J, typename A, bool kRolled = false, typename F>
   __device__ __forceinline__ Found<A> locate(A target, int first, const float (&x)[4 * J], const float (&w)[4 * J], F value) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     A part[J];
+    if constexpr (kRolled) {
+      float copy[4 * J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      A v = A(0);
+      for (int e = 0; e < 4 * J; ++e) copy[e] = x[e];
+#pragma unroll 1
+      for (int j = 0; j < J; ++j)
+        part[j] = (value(copy[4 * j], 0.f) + value(copy[4 * j + 1], 0.f)) + (value(copy[4 * j + 2], 0.f) + value(copy[4 * j + 3], 0.f));
+      A all = A(0);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v += value(x[4 * j + q], w[4 * j + q]);
-      part[j] = v;
+      for (int j = 0; j < J; ++j) all += part[j];
+      target = target * reduce<kSum>(Pass<A>{all, 0, 0.f, 0.f}).sum;
+    } else {
+#pragma unroll
+     for (int j = 0; j < J; ++j) {
+      auto v = value(x[4 * j], w[4 * j]);
+#pragma unroll
+      for (int q = 1; q < 4; ++q) v += value(x[4 * j + q], w[4 * j + q]);
+      part[j] = (A)v;
+     }
     }
     Found<A> f{-1, A(0), A(0)};
     if constexpr (kWarps == 1) {
@@ -255,7 +326,7 @@ template <int kWarps, int kCtas> struct Team {
     int at = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const A v = value(xs[q], ws[q]);
+      const A v = (A)value(xs[q], ws[q]);
       if (v > A(0) && (q == 0 || !(c > target))) { before = c; c += v; at = q; }
     }
     Found<A> f;
@@ -275,13 +346,41 @@ __device__ __forceinline__ float middle_by_bits(float a, float b) {
   return __int_as_float(k >= 0 ? k : (int)0x80000000 - k);
 }
 
-// The weight in 64 bits; a call, because few rows need it and it would be inlined once per element.
-__device__ __noinline__ double exact_weight(float x, float top, float temperature) {
-  return x > -inf_f() ? exp(((double)x - (double)top) / (double)temperature) : 0.0;
+// exp(x) for x <= 0 in double, to a few units of its last place: x = k ln 2 + r with
+// |r| <= ln 2 / 2, the Taylor series of e^r to the 13th power (the next term is below 2^-57),
+// and 2^k by the exponent field. Below e^-700 it is 0.
+__device__ __forceinline__ double exp_below_zero(double x) {
+  if (x < -700.0) return 0.0;
+  const double k = rint(x * 1.4426950408889634074);
+  double r = fma(k, -0.693147180559945309417, x);       // ln 2 rounded to double ...
+  r = fma(k, -2.3190468138462996e-17, r);               // ... and what the rounding left out
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __longlong_as_double(__double_as_longlong(p) + ((long long)k << 52));
 }
 
+// The weight in 64 bits.  Few rows ask for it, so where it is taken for every element the
+// loop runs over groups of four (independent of each other: one waits while the next is
+// worked on) and is not unrolled further; single elements make a call.
+__device__ __forceinline__ double exact_weight(float x, float top, double inverse_t) {
+  return x > -inf_f() ? exp_below_zero(((double)x - (double)top) * inverse_t) : 0.0;
+}
+__device__ __noinline__ double exact_weight_call(float x, float top, double inverse_t) { return exact_weight(x, top, inverse_t); }
+
 template <typename T, int kWarps, int kCtas, int J, int kRowsPerBlock>
-__global__ void __launch_bounds__(kWarps * 32 * kRowsPerBlock)
+__global__ void __launch_bounds__(kWarps * 32 * kRowsPerBlock, kWarps == 1 ? (J <= 4 ? 6 : 4) : (kWarps == 8 ? 2 : 1))
 sample_kernel(const SampleArgs a) {
   constexpr int E = 4 * J;
   using TeamT = Team<kWarps, kCtas>;
@@ -327,20 +426,13 @@ sample_kernel(const SampleArgs a) {
   const float min_p = a.min_p ? __ldg(a.min_p + row) : a.min_p_all;
   const int top_k = a.top_k ? __ldg(a.top_k + row) : a.top_k_all;
 
-  // largest logit, least finite one, how many are not -inf; a NaN counts as +inf
-  Pass<float> p{0.f, 0, inf_f(), -inf_f()};
+  // the largest logit; a NaN anywhere makes it a NaN
+  float most = -inf_f();
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (x[e] != x[e]) x[e] = inf_f();
-    if (x[e] > -inf_f()) { ++p.count; p.least = fminf(p.least, x[e]); }
-    p.most = fmaxf(p.most, x[e]);
-  }
-  p = team.template reduce<kCount | kEnds>(p);
-  const float top = p.most;
-  float least = p.least;
-  const int live = p.count;
-  // (the negations are false for a NaN too)
-  const bool valid = top < inf_f() && live > 0 && temperature >= 0.f && temperature <= 1e6f && top_p == top_p &&
+  for (int e = 0; e < E; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(most) : "f"(most), "f"(x[e]));
+  const float top = team.max_with_nan(most);
+  // (the comparisons are false for a NaN too)
+  const bool valid = top < inf_f() && top > -inf_f() && temperature >= 0.f && temperature <= 1e6f && top_p == top_p &&
                      min_p == min_p && u >= 0.f && u <= 1.f;
   const bool writer = tid == 0 && first == 0;
   if (!valid) {
@@ -356,115 +448,271 @@ sample_kernel(const SampleArgs a) {
     return;
   }
 
-  const float factor = (float)(1.4426950408889634074 / (double)temperature);
-  const auto weight = [&](float y) { const float d = y - top; return d == 0.f ? 1.f : ex2_approx(d * factor); };
-  const auto exact = [&](float y) { return exact_weight(y, top, temperature); };
+  const double inverse_t = 1.0 / (double)temperature;
+  const double factor64 = fmin(1.4426950408889634074 * inverse_t, 3e38);  // exponent = (x - max) * factor
+  const float factor = (float)factor64, lowest = -200.f / factor;         // 2^-200 is 0 in float
+  const float factor_rest = (float)(factor64 - (double)factor);
+  const auto weight = [&](float y) {
+    const float d0 = y - top, d = fmaxf(d0, lowest), t = d * factor;
+    if constexpr (kWarps == 1) return ex2_approx(t);
+    // what the roundings of the subtraction, the factor and the product left out
+    const float b = d0 - y, lost = d0 >= lowest ? (y - (d0 - b)) - (top + b) : 0.f;
+    const float rest = fmaf(lost, factor, fmaf(d, factor_rest, fmaf(d, factor, -t)));
+    const float v = ex2_approx(t);
+    return fmaf(v * 0.6931471805599453f, rest, v);
+  };
+  const auto exact = [&](float y) { return exact_weight_call(y, top, inverse_t); };
   float w[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) w[e] = weight(x[e]);
+  // The sum of f over the thread's elements: in wide rows fours in float, those in double
+  using S = typename TeamT::Sum;
+  const auto sum_of = [&](auto f) {
+    if constexpr (kWarps == 1) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < E; ++e) c[e & 3] += f(e);
+      return (c[0] + c[1]) + (c[2] + c[3]);
+    } else {
+      double c = 0.0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) c += (double)((f(4 * j) + f(4 * j + 1)) + (f(4 * j + 2) + f(4 * j + 3)));
+      return c;
+    }
+  };
+  const auto least_finite = [&]() {
+    Pass<float> r{0.f, 0, inf_f(), 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) r.least = x[e] > -inf_f() ? fminf(r.least, x[e]) : r.least;
+    return team.template reduce<kEnds>(r).least;
+  };
+  // All weights, and those of the logits above `border`, in double.  The loop is not unrolled:
+  // few rows come here, and the code of the others should stay small.
+  const auto exact_sums = [&](float border, double &above) {
+    float copy[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) copy[e] = x[e];
+    double all = 0.0, part = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < J; ++j) {
+      double v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = exact_weight(copy[4 * j + q], top, inverse_t);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        all += v[q];
+        if (copy[4 * j + q] > border) part += v[q];
+      }
+    }
+    above = team.template reduce<kSum>(Pass<double>{part, 0, 0.f, 0.f}).sum;
+    return team.template reduce<kSum>(Pass<double>{all, 0, 0.f, 0.f}).sum;
+  };
   const auto drop = [&](int e) { x[e] = -inf_f(); w[e] = 0.f; };
   const auto index = [&](int e) { return first + 4 * ((e >> 2) * kWarps * 32 + tid) + (e & 3); };
 
   // Keeps the logits above `border` and the first `ties` (by index) of the `equal` that are the border.
   const auto cut = [&](float border, int ties, int equal) {
-    int last = 0x7fffffff;
     if (ties < equal) {
       const auto is_border = [&](float y, float) { return y == border ? 1 : 0; };
-      last = team.template locate<J, int>(ties - 1, first, x, x, is_border).index;
+      const int last = team.template locate<J, int>(ties - 1, first, x, x, is_border).index;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (x[e] == border && index(e) > last) drop(e);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (x[e] < border || (x[e] == border && index(e) > last)) drop(e);
+      if (x[e] < border) drop(e);
+  };
+  const auto equal_to = [&](float y) {
+    Pass<float> c{0.f, 0, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) c.count += x[e] == y;
+    return team.template reduce<kCount>(c).count;
+  };
+  // How many logits lie in (lo, hi], or [lo, hi] if not `open`, the least and the largest of them.
+  const auto between = [&](float lo, float hi, bool open) {
+    const float from = open ? lo : -inf_f();  // not open: lo is the least of all
+    Pass<float> q{0.f, 0, inf_f(), -inf_f()};
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] > from && x[e] <= hi) { ++q.count; q.least = fminf(q.least, x[e]); q.most = fmaxf(q.most, x[e]); }
+    return team.template reduce<kCount | kEnds>(q);
   };
   const auto middle = [&](float lo, float hi, int step) {
     float m = step < 24 ? 0.5f * lo + 0.5f * hi : middle_by_bits(lo, hi);
     return m < hi && m >= lo ? m : lo;
   };
 
+  // One step of a search for a border between lo and hi: kPivots logits evenly between them,
+  // and for each what lies above it in all (weights, or counts).  A lane gets that of the
+  // pivot Team::mine() names; the sums fall from pivot to pivot, so the number of them that
+  // reach the goal says where the border is.
+  constexpr int K = TeamT::kPivots;
+  const int lane = threadIdx.x & 31;
+  const auto pivot = [&](float lo, float hi, int k) { return fminf(lo + (hi - lo) * ((float)(k + 1) / (K + 1)), hi); };
+  const auto lane_of = [](int k) { return TeamT::mine(k); };  // its own inverse
+  constexpr int kSteps = 16;
+
+  float least = -inf_f();  // of the logits kept so far, once a filter has asked for it
+  int live = 0;
+  if (top_k > 0 && top_k < a.V) {
+    Pass<float> r{0.f, 0, inf_f(), 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] > -inf_f()) { ++r.count; r.least = fminf(r.least, x[e]); }
+    r = team.template reduce<kCount | kEnds>(r);
+    least = r.least;
+    live = r.count;
+  }
   if (top_k > 0 && top_k < live) {
-    // border: the logit with fewer than k above it and k at or above it; always in [lo, hi]
-    float lo = least, hi = top;
-    int above = 0;  // logits above hi
+    // border: the logit with fewer than k above it and k at or above it
+    float lo = least, hi = top, found = 0.f;  // found: a border at or above which exactly k lie
+    int above = 0, at_lo = live;              // logits above hi, and at or above lo
     bool split = false;
-    for (int step = 0; lo < hi && !split; ++step) {
-      const float mid = middle(lo, hi, step);
-      Pass<float> r{0.f, 0, inf_f(), -inf_f()};
+    const float goal = (float)top_k;          // counts stay below 2^24: exact
+    bool open = false;                        // lo itself no longer counts
+    for (int step = 0; step < kSteps && at_lo - above > 1 && hi - lo < 1e30f && !split; ++step) {
+      const float was_lo = lo, was_hi = hi;
+      if constexpr (K == 1) {
+        const float mid = pivot(lo, hi, 0);
+        int c[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (x[e] > mid) { ++r.count; r.least = fminf(r.least, x[e]); }
-        else r.most = fmaxf(r.most, x[e]);
+        for (int e = 0; e < E; ++e) c[e & 1] += x[e] > mid;
+        const int n = team.template reduce<kCount>(Pass<float>{0.f, c[0] + c[1], 0.f, 0.f}).count;
+        if (n >= top_k) { lo = mid; at_lo = n; open = true; } else { hi = mid; above = n; }
+      } else {
+        float v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const float pk = pivot(lo, hi, k);
+          int c = 0;
+#pragma unroll
+          for (int e = 0; e < E; ++e) c += x[e] > pk;
+          v[k] = (float)c;
+        }
+        const float n = team.sum_each(v);
+        const int m = __popc(__ballot_sync(kFull, n >= goal) & ((1u << K) - 1u));
+        if (m > 0) { lo = pivot(was_lo, was_hi, m - 1); at_lo = (int)__shfl_sync(kFull, n, lane_of(m - 1)); open = true; }
+        if (m < K) { hi = pivot(was_lo, was_hi, m); above = (int)__shfl_sync(kFull, n, lane_of(m)); }
       }
-      r = team.template reduce<kCount | kEnds>(r);
-      if (r.count >= top_k) lo = r.least; else { hi = r.most; above = r.count; }
-      split = r.count == top_k;
+      split = open && at_lo == top_k;
+      found = lo;
+      if (!(lo > was_lo || hi < was_hi)) break;
     }
-    if (split) {  // exactly k logits at or above lo
-      cut(lo, 1, 1);
-      least = lo;
-    } else {
-      Pass<float> r{0.f, 0, 0.f, 0.f};
+    if (split) {  // exactly k logits above lo
 #pragma unroll
-      for (int e = 0; e < E; ++e) r.count += x[e] == hi;
-      r = team.template reduce<kCount>(r);
-      cut(hi, top_k - above, r.count);
+      for (int e = 0; e < E; ++e)
+        if (!(x[e] > found)) drop(e);
+      least = least_finite();
+    } else {
+      // the logits still in question, from least to most; then bisection between them
+      Pass<float> r = between(lo, hi, open);
+      lo = r.least;
+      hi = r.most;
+      for (int step = 0; lo < hi; ++step) {
+        const float mid = middle(lo, hi, step);
+        Pass<float> b{0.f, 0, inf_f(), -inf_f()};
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (x[e] > mid) { ++b.count; b.least = fminf(b.least, x[e]); }
+          else b.most = fmaxf(b.most, x[e]);
+        }
+        b = team.template reduce<kCount | kEnds>(b);
+        if (b.count >= top_k) lo = b.least; else { hi = b.most; above = b.count; }
+      }
+      cut(hi, top_k - above, r.count == 1 ? 1 : equal_to(hi));
       least = hi;
     }
   }
 
   if (top_p < 1.f) {
-    Pass<float> r{0.f, 0, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < E; ++e) r.sum += w[e];
-    r = team.template reduce<kSum>(r);
-    const float goal = top_p * r.sum, near = 2.f * a.eps * r.sum;
-    double goal64 = -1.0;  // taken only when a comparison needs it
-    const auto exact_sum_above = [&](float border) {
-      Pass<double> d{0.0, 0, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (x[e] > border) d.sum += exact(x[e]);
-      return team.template reduce<kSum>(d).sum;
-    };
+    if (!(least > -inf_f())) least = least_finite();
+    const S total = team.template reduce<kSum>(Pass<S>{sum_of([&](int e) { return w[e]; }), 0, 0.f, 0.f}).sum;
+    const S goal = (S)top_p * total, near = (S)(2.f * a.eps) * total;
     // border: the logit with less than `goal` above it and at least that at or above it
-    float lo = least, hi = top, above = 0.f;
+    float lo = least, hi = top;
+    S above = S(0), at_lo = total;
+    bool above_is_coarse = false;  // from the first search
+    bool open = false;  // lo itself no longer counts
+    if (S(1) - goal > near) {
+      lo = nextafterf(top, -inf_f());  // the largest alone weighs enough: nothing else is in question
+      at_lo = S(0);
+      open = true;
+    } else {
+      // V logits of weight (1 - top_p) * sum / (2 V) each would not weigh what top_p leaves:
+      // the border lies above them
+      const float floor_x = top + temperature * logf((1.f - top_p) * (float)total / (2.f * (float)a.V));
+      if (floor_x > lo) { lo = floor_x; open = true; }
+    }
+    // First by value, as far as float sums decide (their error: that of a row of 1024 at
+    // most); (at_lo - above) / w(hi) is about the number of logits left between.
+    const float coarse = fmaxf((float)near, 2.f * a.eps_steps * (float)total);
+    for (int step = 0; step < kSteps && lo < hi && hi - lo < 1e30f && (float)(at_lo - above) > 1.5f * weight(hi); ++step) {
+      float v[K], at[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) at[k] = pivot(lo, hi, k);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (x[e] > at[k]) c[e & 3] += w[e];
+        v[k] = (c[0] + c[1]) + (c[2] + c[3]);
+      }
+      const float was_lo = lo, was_hi = hi;
+      const float n = team.sum_each(v);
+      if constexpr (K == 1) {
+        if (n >= (float)goal + coarse) { lo = at[0]; at_lo = n; open = true; }        // surely enough above it
+        else if (n <= (float)goal - coarse) { hi = at[0]; above = n; above_is_coarse = kWarps > 1; }  // surely not
+        else break;
+      } else {
+        const int m = __popc(__ballot_sync(kFull, n >= (float)goal + coarse) & ((1u << K) - 1u));
+        const int l = __popc(__ballot_sync(kFull, n > (float)goal - coarse) & ((1u << K) - 1u));
+        if (m > 0) { lo = pivot(was_lo, was_hi, m - 1); at_lo = __shfl_sync(kFull, n, lane_of(m - 1)); open = true; }
+        if (l < K) { hi = pivot(was_lo, was_hi, l); above = __shfl_sync(kFull, n, lane_of(l)); above_is_coarse = true; }
+      }
+      if (!(lo > was_lo || hi < was_hi)) break;
+    }
+    // Then between the logits that are left, from the least to the largest of them.
+    const Pass<float> q = between(lo, hi, open);
+    lo = q.least;
+    hi = q.most;
     for (int step = 0; lo < hi; ++step) {
       const float mid = middle(lo, hi, step);
-      Pass<float> s{0.f, 0, inf_f(), -inf_f()};
+      Pass<S> s{sum_of([&](int e) { return x[e] > mid ? w[e] : 0.f; }), 0, inf_f(), -inf_f()};
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (x[e] > mid) { s.sum += w[e]; s.least = fminf(s.least, x[e]); }
+        if (x[e] > mid) s.least = fminf(s.least, x[e]);
         else s.most = fmaxf(s.most, x[e]);
       }
       s = team.template reduce<kSum | kEnds>(s);
       bool enough = s.sum >= goal;
-      if (fabsf(s.sum - goal) <= near) {
-        if (goal64 < 0.0) goal64 = (double)top_p * exact_sum_above(-inf_f());
-        enough = exact_sum_above(mid) >= goal64;
+      if ((s.sum > goal ? s.sum - goal : goal - s.sum) <= near) {
+        double above64;
+        const double goal64 = (double)top_p * exact_sums(mid, above64);
+        enough = above64 >= goal64;
       }
-      if (enough) lo = s.least; else { hi = s.most; above = s.sum; }
+      if (enough) lo = s.least; else { hi = s.most; above = s.sum; above_is_coarse = false; }
     }
-    Pass<float> c{0.f, 0, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < E; ++e) c.count += x[e] == hi;
-    c = team.template reduce<kCount>(c);
+    const int equal = q.count == 1 ? 1 : equal_to(hi);
     int ties = 1;
-    if (c.count > 1) {
+    if (equal > 1) {
+      if (above_is_coarse) above = team.template reduce<kSum>(Pass<S>{sum_of([&](int e) { return x[e] > hi ? w[e] : 0.f; }), 0, 0.f, 0.f}).sum;
       // the i-th of the border's equals stays while above + i * w < goal
-      const float wb = weight(hi);
-      const float n = ceilf((goal - above) / wb);
-      ties = (int)fminf(fmaxf(n, 1.f), (float)c.count);
-      const float at = above + (float)ties * wb;
-      if (fabsf(at - goal) <= near || (ties > 1 && fabsf(at - wb - goal) <= near) || !(wb > 0.f)) {
-        if (goal64 < 0.0) goal64 = (double)top_p * exact_sum_above(-inf_f());
-        const double above64 = exact_sum_above(hi), wb64 = exact(hi);
+      const S wb = (S)weight(hi), n = ceil((goal - above) / wb);
+      ties = (int)fmin(fmax(n, S(1)), (S)equal);
+      const S at = above + (S)ties * wb - goal;
+      if (!(wb > S(0)) || fabs(at) <= near || (ties > 1 && fabs(at - wb) <= near)) {
+        double above64;
+        const double goal64 = (double)top_p * exact_sums(hi, above64), wb64 = exact(hi);
         double m = ceil((goal64 - above64) / wb64);
-        m = fmin(fmax(m, 1.0), (double)c.count);  // a NaN (0 / 0) becomes 1
+        m = fmin(fmax(m, 1.0), (double)equal);  // a NaN (0 / 0) becomes 1
         if (m > 1.0 && above64 + (m - 1.0) * wb64 >= goal64) m -= 1.0;
-        else if (m < (double)c.count && above64 + m * wb64 < goal64) m += 1.0;
+        else if (m < (double)equal && above64 + m * wb64 < goal64) m += 1.0;
         ties = (int)m;
       }
     }
-    cut(hi, ties, c.count);
+    cut(hi, ties, equal);
   }
 
   if (min_p > 0.f) {
@@ -478,23 +726,16 @@ sample_kernel(const SampleArgs a) {
     }
   }
 
-  Pass<float> z{0.f, 0, 0.f, 0.f};
-#pragma unroll
-  for (int e = 0; e < E; ++e) z.sum += w[e];
-  z = team.template reduce<kSum>(z);
-  const float goal = u * z.sum, near = 2.f * a.eps * z.sum;
+  const S sum = team.template reduce<kSum>(Pass<S>{sum_of([&](int e) { return w[e]; }), 0, 0.f, 0.f}).sum;
+  const S goal = (S)u * sum, near = (S)(2.f * a.eps) * sum;
   const auto value = [](float, float v) { return v; };
-  const auto f = team.template locate<J, float>(goal, first, x, w, value);
+  const auto f = team.template locate<J, S>(goal, first, x, w, value);
   int token = f.index;
   if (token < 0 || f.upto - goal <= near || goal - f.before <= near) {
-    Pass<double> d{0.0, 0, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < E; ++e) d.sum += exact(x[e]);
-    const double total = team.template reduce<kSum>(d).sum;
-    const auto value64 = [&](float y, float) { return exact(y); };
+    const auto value64 = [&](float y, float) { return exact_weight(y, top, inverse_t); };
     // u = 1 asks for the last: two orders of adding the same doubles may differ by a
     // rounding, which is far below the 2^-24 that any other u stays away from the total
-    token = u < 1.f ? team.template locate<J, double>((double)u * total, first, x, w, value64).index : -1;
+    token = u < 1.f ? team.template locate<J, double, true>((double)u, first, x, w, value64).index : -1;
     if (token < 0) {  // the last that has any weight (indices stay below 2^24: exact in float)
       Pass<float> last{0.f, 0, 0.f, -1.f};
 #pragma unroll
@@ -506,7 +747,7 @@ sample_kernel(const SampleArgs a) {
   if (tid == 0 && first == 0) {
     const float xt = to_float(src[token]);
     a.token[row] = token;
-    a.logprob[row] = (xt - top) / temperature - logf(z.sum);
+    a.logprob[row] = (xt - top) / temperature - logf((float)sum);
   }
   if constexpr (kCtas > 1) cg::this_cluster().sync();  // no block leaves while another reads its shared memory
 }
@@ -523,7 +764,11 @@ int fail(int code, const char *fmt, ...) {
 
 template <typename T, int kWarps, int kCtas, int J, int kRowsPerBlock>
 cudaError_t launch(SampleArgs a, cudaStream_t s) {
-  a.eps = (3.f * logf((float)a.V + 2.f) + 4 * J + 24) * 5.9604645e-8f;
+  // additions on the longest path of a warp's row: J in a chain, 2 to join four, 5 in the warp, and u * sum;
+  // of a wide row's first search also 5 and 3 across warps and blocks
+  const float ulp = 5.9604645e-8f, ln_v = logf((float)a.V + 2.f);
+  a.eps = kWarps == 1 ? (3.f * ln_v + (J + 2 + 5 + 1) + 6) * ulp : 9.f * ulp;
+  a.eps_steps = (3.f * ln_v + (J + 2 + 5 + 5 + 3) + 8) * ulp;
   cudaLaunchConfig_t cfg = {};
   const int64_t blocks = kWarps == 1 ? (a.rows + kRowsPerBlock - 1) / kRowsPerBlock : a.rows * kCtas;
   if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
@@ -548,6 +793,7 @@ template <typename T> cudaError_t launch_by_width(const SampleArgs &a, cudaStrea
   if (a.V <= 512) return launch<T, 1, 1, 4, 4>(a, s);
   if (a.V <= 1024) return launch<T, 1, 1, 8, 4>(a, s);
   if (a.V <= 4096) return launch<T, 8, 1, 4, 1>(a, s);
+  if (a.V <= 6144) return launch<T, 8, 1, 6, 1>(a, s);
   if (a.V <= 8192) return launch<T, 16, 1, 4, 1>(a, s);
   if (a.V <= 16384) return launch<T, 16, 1, 8, 1>(a, s);
   if (a.V <= 65536) return launch<T, 16, 8, 4, 1>(a, s);
