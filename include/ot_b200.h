@@ -384,6 +384,16 @@ int ot_b200_clip_gradients(int32_t n, const void *const *grads, const int64_t *c
                            double max_norm, void *d_workspace, uint64_t workspace_bytes, float *d_norm,
                            void *stream);
 
+/* Both in one call for the forward pass: d_out (rows, V) = x * w^T (+ bias) with x (rows, D)
+ * of the type x_flags says, quantised in blocks of 1 x 128 into the workspace (256-byte
+ * aligned), and w (V, D) a quantised `b` as above.  out_flags: the flags of
+ * ot_b200_fp8_matmul. */
+int ot_b200_joiner_logits_workspace_bytes(int64_t rows, int32_t D, int32_t V, uint64_t *bytes_out);
+int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_stride, uint32_t x_flags,
+                          const void *d_w, int64_t w_pitch, const float *d_w_scale, int32_t V,
+                          const float *d_bias, uint32_t out_flags, void *d_workspace,
+                          uint64_t workspace_bytes, void *d_out, void *stream);
+
 /* d_grad[i] *= *d_scale for i < count, unless *d_scale == 1 (then the buffer is
  * not touched: the kernel's blocks return after one load).  The counterpart of
  * `ctx.grad.mul_(loss_grad)` (transducer_loss.py:162) for a gradient that

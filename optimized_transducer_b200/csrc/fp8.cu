@@ -843,4 +843,38 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
   return OT_B200_OK;
 }
 
+// x in e4m3, its scales, and the product's own workspace, one behind the other.
+static void joiner_layout(int64_t rows, int64_t D, uint64_t *scale_off, uint64_t *product_off) {
+  const auto align = [](uint64_t n) { return (n + 255) & ~uint64_t(255); };
+  *scale_off = align((uint64_t)rows * ((D + 15) / 16 * 16));
+  *product_off = *scale_off + align((uint64_t)rows * ((D + kScaleBlock - 1) / kScaleBlock) * sizeof(float));
+}
+
+int ot_b200_joiner_logits_workspace_bytes(int64_t rows, int32_t D, int32_t V, uint64_t *bytes_out) {
+  uint64_t product = 0, scale_off, product_off;
+  const int rc = ot_b200_fp8_matmul_workspace_bytes(rows, V, D, &product);
+  if (rc) return rc;
+  joiner_layout(rows, D, &scale_off, &product_off);
+  *bytes_out = product_off + product;
+  return OT_B200_OK;
+}
+
+int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_stride, uint32_t x_flags, const void *d_w,
+                          int64_t w_pitch, const float *d_w_scale, int32_t V, const float *d_bias, uint32_t out_flags,
+                          void *d_workspace, uint64_t workspace_bytes, void *d_out, void *stream) {
+  uint64_t need = 0, scale_off, product_off;
+  int rc = ot_b200_joiner_logits_workspace_bytes(rows, D, V, &need);
+  if (rc) return rc;
+  if (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0)
+    return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_logits: workspace missing, not 256-byte aligned or smaller than %llu bytes", (unsigned long long)need);
+  joiner_layout(rows, D, &scale_off, &product_off);
+  char *ws = static_cast<char *>(d_workspace);
+  const int64_t pitch = ((int64_t)D + 15) / 16 * 16;
+  float *scale = reinterpret_cast<float *>(ws + scale_off);
+  rc = ot_b200_fp8_quantize(d_x, rows, D, row_stride, x_flags, OT_B200_FP8_ROWS, ws, pitch, scale, nullptr, 0, nullptr, nullptr, nullptr, stream);
+  if (rc) return rc;
+  return ot_b200_fp8_matmul(ws, pitch, scale, d_w, w_pitch, d_w_scale, d_bias, rows, V, D, out_flags,
+                            ws + product_off, workspace_bytes - product_off, d_out, stream);
+}
+
 }  // extern "C"

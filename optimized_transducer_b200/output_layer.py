@@ -38,6 +38,39 @@ def _stream(device):
     return torch.cuda.current_stream(device.index).cuda_stream
 
 
+_WORKSPACE = {}  # (rows, D, V) -> bytes: a decoder's shapes repeat from step to step
+
+
+def _workspace_bytes(lib, rows, d, v):
+    key = (rows, d, v)
+    n = _WORKSPACE.get(key)
+    if n is None:
+        if len(_WORKSPACE) >= 256:
+            _WORKSPACE.clear()
+        need = ctypes.c_uint64()
+        _lib.check(lib.ot_b200_joiner_logits_workspace_bytes(rows, d, v, ctypes.byref(need)))
+        n = _WORKSPACE[key] = need.value
+    return n
+
+
+def _forward(x, w, pitch, scale, bias, v, out_dtype):
+    """The logits of a quantised weight, (rows, V): one library call."""
+    rows, d = x.shape
+    dev = x.device
+    lib = _lib.load()
+    size = _workspace_bytes(lib, rows, d, v)
+    out = torch.empty((rows, v), dtype=out_dtype, device=dev)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    flags = _DTYPE_FLAG[out_dtype] | (0 if _check_mode() == "off" else _lib.REPORT_ERRORS)
+    with _on_device(dev.index):
+        rc = lib.ot_b200_joiner_logits(
+            x.data_ptr(), rows, d, x.stride(0) if rows > 1 else d, _DTYPE_FLAG[x.dtype], w.data_ptr(), pitch, scale.data_ptr(), v,
+            bias.data_ptr() if bias is not None else None, flags, ws.data_ptr(), size, out.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc)
+    return out
+
+
 class Fp8Weight:
     """A quantised projection weight.  ``data``: (V, D) ``torch.float8_e4m3fn``, unit
     column stride, rows a multiple of 16 bytes apart, 16-byte aligned; ``scale``:
@@ -48,6 +81,12 @@ class Fp8Weight:
 
     def __init__(self, data, scale):
         who = "Fp8Weight"
+        if (data.dtype is torch.float8_e4m3fn and data.is_cuda and data.is_contiguous() and data.dim() == 2
+                and data.size(1) % 16 == 0 and data.numel() > 0 and data.data_ptr() % 16 == 0
+                and scale.dtype is torch.float32 and scale.is_contiguous() and scale.device == data.device
+                and scale.shape == (_blocks(data.size(0)), _blocks(data.size(1)))):
+            self.data, self.scale = data, scale  # the common case: one pass over the metadata
+            return
         if data.dtype != torch.float8_e4m3fn or data.dim() != 2 or data.numel() == 0:
             raise RuntimeError(f"{who}: data must be a non-empty 2-D float8_e4m3fn tensor")
         if not data.is_cuda:
@@ -189,8 +228,29 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     so overwriting ``joiner_in`` afterwards does no harm.  An :class:`Fp8Weight` has
     no gradient: ``joiner_in`` may then not require one."""
     who = "joiner_logits"
-    _check_matrix(joiner_in, "joiner_in", who)
     served = isinstance(weight, Fp8Weight)
+    w = weight.data if served else weight
+    grads = torch.is_grad_enabled() and (joiner_in.requires_grad or (bias is not None and bias.requires_grad)
+                                         or (not served and weight.requires_grad))
+    if not (served and not grads and joiner_in.is_cuda and joiner_in.is_contiguous() and joiner_in.dim() == 2
+            and joiner_in.dtype in _FLOATS and out_dtype in _FLOATS and w.device == joiner_in.device
+            and joiner_in.size(1) == w.size(1) and joiner_in.size(0) > 0
+            and (bias is None or (bias.dtype is torch.float32 and bias.dim() == 1 and bias.is_contiguous()
+                                  and bias.size(0) == w.size(0) and bias.device == joiner_in.device))):
+        _check_arguments(joiner_in, weight, bias, out_dtype, served, grads, who)
+        if joiner_in.size(0) == 0:
+            return torch.empty((0, w.size(0)), dtype=out_dtype, device=joiner_in.device)
+        if grads:
+            return JoinerLogitsFunction.apply(joiner_in, weight, bias, out_dtype)
+    if served:
+        return _forward(joiner_in, w, w.stride(0) if w.size(0) > 1 else _pitch(w.size(1)), weight.scale, bias, w.size(0), out_dtype)
+    q, scale = _quantize(weight, _lib.FP8_SQUARES)[0]
+    return _forward(joiner_in, q, q.size(1), scale, bias, weight.size(0), out_dtype)
+
+
+def _check_arguments(joiner_in, weight, bias, out_dtype, served, grads, who):
+    """Raises the error for the first argument of :func:`joiner_logits` that will not do."""
+    _check_matrix(joiner_in, "joiner_in", who)
     if not served:
         _check_matrix(weight, "weight", who)
     if weight.device != joiner_in.device or weight.shape[1] != joiner_in.size(1) or weight.shape[0] == 0:
@@ -201,17 +261,7 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
         raise RuntimeError(f"{who}: bias must be a contiguous float32 tensor of V entries")
     if out_dtype not in _FLOATS:
         raise RuntimeError(f"{who}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    grads = torch.is_grad_enabled() and (joiner_in.requires_grad or (bias is not None and bias.requires_grad)
-                                         or (not served and weight.requires_grad))
     if served and grads:
         raise RuntimeError(f"{who}: an Fp8Weight is for inference; pass the weight as a tensor to train")
-    rows, d = joiner_in.shape
-    if rows == 0:
-        if grads:
-            raise RuntimeError(f"{who}: joiner_in has no rows")
-        return torch.empty((0, weight.shape[0]), dtype=out_dtype, device=joiner_in.device)
-    if grads:
-        return JoinerLogitsFunction.apply(joiner_in, weight, bias, out_dtype)
-    w = (weight.data, weight.scale) if served else _quantize(weight.detach(), _lib.FP8_SQUARES)[0]
-    x, _, _ = _quantize(joiner_in.detach(), _lib.FP8_ROWS)
-    return _matmul(x, w, rows, weight.shape[0], d, out_dtype, bias.detach() if bias is not None else None)
+    if grads and joiner_in.size(0) == 0:
+        raise RuntimeError(f"{who}: joiner_in has no rows")

@@ -13,6 +13,7 @@ from .transducer_loss import _DTYPE_FLAG, _on_device
 __all__ = ["sample_tokens"]
 
 MAX_V = 262144
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _setting(value, name, dtype, logits):
@@ -44,37 +45,49 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     without a finite maximum (everything ``-inf``, or a NaN or ``+inf`` in it), or whose
     own settings are out of range (``uniforms`` outside [0, 1], ``temperature`` outside
     [0, 1e6], a NaN), gets token -1 and log-probability NaN."""
+    t_ptr, t = (None, temperature) if type(temperature) is float else _setting(temperature, "temperature", torch.float32, logits)
+    k_ptr, k = (None, top_k) if type(top_k) is int else _setting(top_k, "top_k", torch.int32, logits)
+    p_ptr, p = (None, top_p) if type(top_p) is float else _setting(top_p, "top_p", torch.float32, logits)
+    m_ptr, m = (None, min_p) if type(min_p) is float else _setting(min_p, "min_p", torch.float32, logits)
+    if not (logits.is_cuda and logits.dtype in _FLOATS and logits.dim() == 2 and logits.is_contiguous()
+            and 1 <= logits.size(1) <= MAX_V and logits.size(0) > 0 and uniforms.dtype is torch.float32
+            and uniforms.is_contiguous() and uniforms.dim() == 1 and uniforms.size(0) == logits.size(0)
+            and uniforms.device == logits.device and (t_ptr is not None or 0.0 <= t <= 1e6) and p == p and m == m
+            and -0x80000000 <= k <= 0x7fffffff):
+        _check_arguments(logits, uniforms, t_ptr, t, k, p, m)
+    rows, v = logits.shape
+    device = logits.device
+    tokens = torch.empty(rows, dtype=torch.int32, device=device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    if rows == 0:
+        return tokens, logprobs
+    index = device.index
+    with _on_device(index):
+        rc = _lib.load().ot_b200_sample(
+            logits.data_ptr(), rows, v, logits.stride(0) if rows > 1 else v, _DTYPE_FLAG[logits.dtype],
+            uniforms.data_ptr(), t_ptr, t, k_ptr, k, p_ptr, p, m_ptr, m, tokens.data_ptr(), logprobs.data_ptr(),
+            torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        _lib.check(rc)
+    return tokens, logprobs
+
+
+def _check_arguments(logits, uniforms, t_ptr, t, k, p, m):
+    """Raises the error for the first argument of :func:`sample_tokens` that will not do."""
     who = "sample_tokens"
     if not logits.is_cuda:
         raise RuntimeError(f"{who}: CUDA tensors only (sm_100a kernels, no CPU path)")
-    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if logits.dtype not in _FLOATS:
         raise RuntimeError(f"{who}: expected logits to be float32, bfloat16 or float16, got {logits.dtype}")
     if logits.dim() != 2 or not 1 <= logits.size(1) <= MAX_V or (logits.size(1) > 1 and logits.stride(1) != 1) \
             or (logits.size(0) > 1 and logits.stride(0) < logits.size(1)):
         raise RuntimeError(f"{who}: expected logits to be (rows, V) with contiguous rows and 1 <= V <= {MAX_V}")
-    rows, v = logits.shape
-    if uniforms.dtype != torch.float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous() \
+    if uniforms.dtype != torch.float32 or uniforms.shape != (logits.size(0),) or not uniforms.is_contiguous() \
             or uniforms.device != logits.device:
         raise RuntimeError(f"{who}: uniforms must be a contiguous float32 tensor with one value per row on {logits.device}")
-    t_ptr, t = _setting(temperature, "temperature", torch.float32, logits)
-    k_ptr, k = _setting(top_k, "top_k", torch.int32, logits)
-    p_ptr, p = _setting(top_p, "top_p", torch.float32, logits)
-    m_ptr, m = _setting(min_p, "min_p", torch.float32, logits)
     if t_ptr is None and not 0.0 <= t <= 1e6:
         raise RuntimeError(f"{who}: temperature must be in [0, 1e6], got {t}")
     if p != p or m != m:
         raise RuntimeError(f"{who}: top_p and min_p must be numbers")
     if not -(1 << 31) <= k < (1 << 31):
         raise RuntimeError(f"{who}: top_k must fit 32 bits, got {k}")
-    logits = logits.detach()
-    tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    if rows == 0:
-        return tokens, logprobs
-    index = logits.device.index
-    with _on_device(index):
-        _lib.check(_lib.load().ot_b200_sample(
-            logits.data_ptr(), rows, v, logits.stride(0) if rows > 1 else v, _DTYPE_FLAG[logits.dtype],
-            uniforms.data_ptr(), t_ptr, t, k_ptr, k, p_ptr, p, m_ptr, m, tokens.data_ptr(), logprobs.data_ptr(),
-            torch.cuda.current_stream(index).cuda_stream))
-    return tokens, logprobs

@@ -58,3 +58,19 @@ def test_product_argument_errors():
     assert lib.ot_b200_fp8_matmul_workspace_bytes(10, 10, 100000, ctypes.byref(need)) == _lib.OK and need.value > 0
     assert call(**long_k, ws=p, wb=need.value - 1) == _lib.ERR_WORKSPACE
     assert lib.ot_b200_fp8_matmul_workspace_bytes(100000, 500, 512, ctypes.byref(need)) == _lib.OK and need.value == 0
+
+
+def test_forward_in_one_call_argument_errors():
+    lib = _lib.load()
+    keep, p = _memory()
+    need = ctypes.c_uint64()
+    assert lib.ot_b200_joiner_logits_workspace_bytes(0, 20, 5, ctypes.byref(need)) == _lib.ERR_ARGUMENT
+    assert lib.ot_b200_joiner_logits_workspace_bytes(4, 20, 5, ctypes.byref(need)) == _lib.OK and need.value >= 4 * 32 + 16
+
+    def call(x=p, rows=4, d=20, ld=20, xf=0, w=p, wp=32, ws_=p, v=5, of=0, ws=p, wb=need.value, out=p):
+        return lib.ot_b200_joiner_logits(x, rows, d, ld, xf, w, wp, ws_, v, None, of, ws, wb, out, None)
+
+    for kw in (dict(ws=None), dict(ws=p + 16), dict(wb=need.value - 1)):
+        assert call(**kw) == _lib.ERR_WORKSPACE, kw
+    for kw in (dict(x=None), dict(rows=0), dict(d=0), dict(v=0), dict(ld=19), dict(xf=_lib.FP64)):
+        assert call(**kw) == _lib.ERR_ARGUMENT, kw
