@@ -312,7 +312,8 @@ int ot_b200_backward_linear(const void *d_x, const void *d_w, const float *d_bia
  * infinity or a NaN):
  *   d_q      (rows, cols) bytes, rows q_pitch bytes apart (a multiple of 16; base 16-byte aligned)
  *   d_scale  blocks of 1 x 128: [ceil(cols/128)][rows];  128 x 128: [ceil(rows/128)][ceil(cols/128)]
- *   d_qt     (cols, rows) bytes, rows qt_pitch = rows rounded up to 16 bytes apart, or NULL
+ *   d_qt     (cols, rows) bytes, rows qt_pitch bytes apart (a multiple of 16, from rows to rows
+ *            rounded up to 128; whole cache lines are the faster ones to read), or NULL
  *   d_scale_t  blocks of 128 x 1 (of x): [ceil(rows/128)][cols];  128 x 128: [ceil(cols/128)][ceil(rows/128)]
  *   d_column_sums  (cols) float sums of x over its rows, or NULL; then d_partial_sums holds
  *            ceil(rows/128) * cols floats of scratch (mode ..._ROWS_AND_COLUMNS only)

@@ -653,10 +653,15 @@ split_sum_kernel(const float *__restrict__ part, int splits, int64_t stride, int
 // ---------------------------------------------------------------------------
 struct MatmulPlan { int tile_n, splits; };
 
+// Rows of one piece's partial sums: whole row tiles, so that a store never reaches the next piece's.
+int64_t whole_tiles(int64_t M) { return (M + kTileM - 1) / kTileM * kTileM; }
+
 // Columns per tile: the widest tile that still gives every SM a tile of its own (per K
 // block a wide tile reads fewer bytes of shared memory per product); a narrower N wants no
-// wider tile.  Pieces of K: only when even then most SMs would idle and K is long (dW: K is
-// the number of rows), at least eight blocks of K each.
+// wider tile.  Pieces of K, when K is long (dW: K is the number of rows): as many as make
+// the shortest of the times below, where a K block of a 256-column tile takes 0.4 us and the
+// pieces' sums are written and read once at 4 TB/s, behind one more launch (80 tiles of 909
+// blocks on 148 SMs: 538 us in one piece, 330 in five).
 MatmulPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
   const int64_t mt = (M + kTileM - 1) / kTileM, kb = (K + kScaleBlock - 1) / kScaleBlock;
   const bool long_k = kb >= 32;
@@ -664,12 +669,16 @@ MatmulPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
   while (tile_n > 64 && (N <= tile_n / 2 || (!long_k && mt * ((N + tile_n - 1) / tile_n) < sms))) tile_n /= 2;
   const int64_t tiles = mt * ((N + tile_n - 1) / tile_n);
   int splits = 1;
-  if (long_k && 2 * tiles <= sms) splits = (int)std::min<int64_t>(sms / tiles, kb / 8);
+  if (long_k && tiles < 2 * sms) {
+    double best = 1e300;
+    for (int s = 1; s <= kb / 8 && s <= 2 * sms; ++s) {
+      const double blocks = (double)((tiles * s + sms - 1) / sms) * (double)((kb + s - 1) / s);
+      const double us = blocks * 0.4 * tile_n / 256 + (s > 1 ? 3.0 + s * (double)whole_tiles(M) * N * 8 / 4e6 : 0.0);
+      if (us < 0.98 * best) { best = us; splits = s; }
+    }
+  }
   return {tile_n, splits};
 }
-
-// Rows of one piece's partial sums: whole row tiles, so that a store never reaches the next piece's.
-int64_t whole_tiles(int64_t M) { return (M + kTileM - 1) / kTileM * kTileM; }
 
 template <int kTileN, typename OutT>
 cudaError_t launch_matmul(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const MatmulArgs &g, cudaStream_t s) {
@@ -733,11 +742,12 @@ int ot_b200_fp8_quantize(const void *d_x, int64_t rows, int32_t cols, int64_t ro
   if (mode < OT_B200_FP8_ROWS || mode > OT_B200_FP8_ROWS_AND_COLUMNS)
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: unknown mode %d", mode);
   const bool with_t = mode == OT_B200_FP8_ROWS_AND_SQUARES || mode == OT_B200_FP8_SQUARES_BOTH || mode == OT_B200_FP8_ROWS_AND_COLUMNS;
-  const int64_t need = (cols + 15) / 16 * 16, need_t = (rows + 15) / 16 * 16;
+  const int64_t need = ((int64_t)cols + 15) / 16 * 16, need_t = (rows + 15) / 16 * 16;
   if (!d_q || !d_scale || !aligned16(d_q) || q_pitch % 16 != 0 || q_pitch < need)
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: q and scale must be non-NULL, q 16-byte aligned, its pitch a multiple of 16 of at least cols");
-  if (with_t && (!d_qt || !d_scale_t || !aligned16(d_qt) || qt_pitch != need_t))
-    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: qt and scale_t must be non-NULL, qt 16-byte aligned, its pitch rows rounded up to 16");
+  if (with_t && (!d_qt || !d_scale_t || !aligned16(d_qt) || qt_pitch % 16 != 0 || qt_pitch < need_t ||
+                 qt_pitch > (rows + kScaleBlock - 1) / kScaleBlock * kScaleBlock))
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: qt and scale_t must be non-NULL, qt 16-byte aligned, its pitch a multiple of 16 from rows to rows rounded up to 128");
   if ((d_partial_sums == nullptr) != (d_column_sums == nullptr) || (d_column_sums && mode != OT_B200_FP8_ROWS_AND_COLUMNS))
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_quantize: column sums come with mode OT_B200_FP8_ROWS_AND_COLUMNS and both of their buffers");
   QuantArgs a;
@@ -843,10 +853,14 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
   return OT_B200_OK;
 }
 
+// Bytes from row to row of a quantised matrix: whole cache lines, so that the 128 bytes of a
+// row that one TMA box takes lie in one line and not in two.
+static int64_t row_pitch(int64_t n) { return (n + 127) / 128 * 128; }
+
 // x in e4m3, its scales, and the product's own workspace, one behind the other.
 static void joiner_layout(int64_t rows, int64_t D, uint64_t *scale_off, uint64_t *product_off) {
   const auto align = [](uint64_t n) { return (n + 255) & ~uint64_t(255); };
-  *scale_off = align((uint64_t)rows * ((D + 15) / 16 * 16));
+  *scale_off = align((uint64_t)rows * row_pitch(D));
   *product_off = *scale_off + align((uint64_t)rows * ((D + kScaleBlock - 1) / kScaleBlock) * sizeof(float));
 }
 
@@ -869,7 +883,7 @@ int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_
     return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_logits: workspace missing, not 256-byte aligned or smaller than %llu bytes", (unsigned long long)need);
   joiner_layout(rows, D, &scale_off, &product_off);
   char *ws = static_cast<char *>(d_workspace);
-  const int64_t pitch = ((int64_t)D + 15) / 16 * 16;
+  const int64_t pitch = row_pitch(D);
   float *scale = reinterpret_cast<float *>(ws + scale_off);
   rc = ot_b200_fp8_quantize(d_x, rows, D, row_stride, x_flags, OT_B200_FP8_ROWS, ws, pitch, scale, nullptr, 0, nullptr, nullptr, nullptr, stream);
   if (rc) return rc;

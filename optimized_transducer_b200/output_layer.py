@@ -31,7 +31,8 @@ def _blocks(n):
 
 
 def _pitch(n):
-    return -(-n // 16) * 16
+    """Bytes from row to row of a quantised matrix: whole cache lines."""
+    return -(-n // 128) * 128
 
 
 def _stream(device):
