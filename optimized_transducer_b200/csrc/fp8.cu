@@ -378,6 +378,13 @@ struct MatmulArgs {
   int32_t seq;
 };
 
+// True for one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 template <int kTileN> struct MatmulShared {
   uint64_t full[Shape<kTileN>::ring];          // TMA -> MMA
   uint64_t empty[Shape<kTileN>::ring];         // MMA -> TMA
@@ -407,7 +414,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   constexpr int R = S::ring, B = S::accumulators;
   extern __shared__ __align__(1024) unsigned char ring_mem[];
   __shared__ MatmulShared<kTileN> sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // one value per warp, for the compiler too
   unsigned char *ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(ring_mem) + 1023) & ~uintptr_t(1023));
   unsigned char *staging = ring + (size_t)R * S::stage_bytes;
 
@@ -451,24 +458,37 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     return p;
   };
 
-  if (warp == 0 && lane == 0) {
-    uint32_t it = 0;
-    for (uint32_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
+  // The two control warps run their loops with all lanes and let one issue: stage indices,
+  // barrier addresses and descriptors then live in uniform registers, where the MMAs want them.
+  // (With one lane in the loop the issue of a block's MMAs took 740 cycles, more than the MMAs.)
+  if (warp == 0) {
+    int s = 0;           // stage
+    uint32_t phase = 1;  // parity of the wait for it; the first round finds the stages empty
+    uint32_t issued = 0;
+    bool dead = false;
+    for (uint32_t tile = blockIdx.x; tile < g.tiles && !dead; tile += gridDim.x) {
       const Place p = place(tile);
-      for (int kb = p.k0; kb < p.k1; ++kb, ++it) {
-        const int s = it % R;
-        if (it >= R && !mbar_wait(&sh.empty[s], ((it / R) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+      for (int kb = p.k0; kb < p.k1; ++kb) {
+        if (issued >= (uint32_t)R) {
+          dead = !__all_sync(kFull, mbar_wait(&sh.empty[s], phase, &sh.abort));
+          if (dead) { sh.abort = 1; break; }
+        }
         unsigned char *a = ring + (size_t)s * S::stage_bytes;
-        mbar_expect_tx(&sh.full[s], S::stage_bytes);
-        // what lies beyond either matrix is filled with zeros by the copy
-        tma_load_2d(a, &map_a, kb * kScaleBlock, p.mt * kTileM, &sh.full[s]);
-        tma_load_2d(a + kBytesA, &map_b, kb * kScaleBlock, p.nt * kTileN, &sh.full[s]);
+        if (elect_one()) {
+          mbar_expect_tx(&sh.full[s], S::stage_bytes);
+          // what lies beyond either matrix is filled with zeros by the copy
+          tma_load_2d(a, &map_a, kb * kScaleBlock, p.mt * kTileM, &sh.full[s]);
+          tma_load_2d(a + kBytesA, &map_b, kb * kScaleBlock, p.nt * kTileN, &sh.full[s]);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == R) { s = 0; phase ^= 1; }
       }
     }
-    if (sh.abort) {
+    if (dead || sh.abort) {
       const volatile int *never = &sh.never;
-      for (uint32_t j = (it > R ? it - R : 0); j < it; ++j) mbar_wait(&sh.full[j % R], (j / R) & 1, never);
-      if (g.sticky != nullptr) {
+      for (uint32_t j = (issued > (uint32_t)R ? issued - R : 0); j < issued; ++j) mbar_wait(&sh.full[j % R], (j / R) & 1, never);
+      if (lane == 0 && g.sticky != nullptr) {
         volatile int32_t *r = g.sticky;
         r[1] = 0;
         r[2] = g.seq;
@@ -476,22 +496,32 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         r[0] = OT_B200_COPY_TIMEOUT;
       }
     }
-  } else if (warp == 1 && lane == 0) {
-    uint32_t it = 0;
-    for (uint32_t tile = blockIdx.x; tile < g.tiles && !sh.abort; tile += gridDim.x) {
+  } else if (warp == 1) {
+    int s = 0, buf = 0;
+    uint32_t full_phase = 0, free_phase = 1, blocks = 0;
+    const uint64_t desc_a = smem_desc(smem_u32(ring)), desc_b = smem_desc(smem_u32(ring) + kBytesA);
+    bool dead = false;
+    for (uint32_t tile = blockIdx.x; tile < g.tiles && !dead; tile += gridDim.x) {
       const Place p = place(tile);
-      for (int kb = p.k0; kb < p.k1; ++kb, ++it) {
-        const int s = it % R, buf = it % B;
-        if (it >= B && !mbar_wait(&sh.acc_empty[buf], ((it / B) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
-        if (!mbar_wait(&sh.full[s], (it / R) & 1, &sh.abort)) { sh.abort = 1; break; }
+      for (int kb = p.k0; kb < p.k1; ++kb, ++blocks) {
+        bool ok = true;
+        if (blocks >= (uint32_t)B) ok = mbar_wait(&sh.acc_empty[buf], free_phase, &sh.abort);
+        ok = ok && mbar_wait(&sh.full[s], full_phase, &sh.abort);
+        dead = !__all_sync(kFull, ok);
+        if (dead) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t a = smem_u32(ring + (size_t)s * S::stage_bytes);
-        const uint64_t da = smem_desc(a), db = smem_desc(a + kBytesA);
+        const uint64_t step = (uint64_t)((uint32_t)s * (S::stage_bytes >> 4));
+        const uint32_t d = tmem + (uint32_t)(buf * kTileN);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kScaleBlock / kMmaK; ++k)  // 32 bytes further along K inside the swizzle row
-          mma_f8(tmem + (uint32_t)(buf * kTileN), da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), S::instr, k != 0);
-        mma_commit(&sh.empty[s]);
-        mma_commit(&sh.acc_full[buf]);
+          for (int k = 0; k < kScaleBlock / kMmaK; ++k)  // 32 bytes further along K inside the swizzle row
+            mma_f8(d, desc_a + step + (uint64_t)(k * 2), desc_b + step + (uint64_t)(k * 2), S::instr, k != 0);
+          mma_commit(&sh.empty[s]);
+          mma_commit(&sh.acc_full[buf]);
+        }
+        __syncwarp();
+        if (++s == R) { s = 0; full_phase ^= 1; }
+        if (++buf == B) { buf = 0; free_phase ^= 1; }
       }
     }
   } else if (warp >= 2) {
