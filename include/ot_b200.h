@@ -395,6 +395,27 @@ int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_
                           const float *d_bias, uint32_t out_flags, void *d_workspace,
                           uint64_t workspace_bytes, void *d_out, void *stream);
 
+/* A training step of the projection: the forward call quantises w (V, D; rows w_stride
+ * elements apart) and x (rows, D) itself and leaves w^T and x^T in e4m3 in d_saved (as far as
+ * the gradients with respect to x and to w are wanted: need_x, need_w); the backward call
+ * takes the gradient g (rows, V) of the logits and writes
+ *   d_gx (rows, D) = q(g) q(w)     d_gw (V, D) = q(g^T) q(x)     d_gb (V) float = column sums of g
+ * each NULL when it is not wanted (need_x, need_w of the forward call must agree with d_gx,
+ * d_gw).  q(g), q(g^T) in blocks of 128 along the contraction, w and x in 128 x 128.  The
+ * three buffers are 256-byte aligned and as large as ot_b200_joiner_train_bytes says for the
+ * same needs; types by flags as above, `flags` may hold OT_B200_REPORT_ERRORS. */
+int ot_b200_joiner_train_bytes(int64_t rows, int32_t D, int32_t V, int32_t need_x, int32_t need_w,
+                               int32_t need_b, uint64_t *saved_out, uint64_t *forward_out,
+                               uint64_t *backward_out);
+int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags,
+                                 const void *d_w, int32_t V, int64_t w_stride, uint32_t w_flags,
+                                 const float *d_bias, uint32_t out_flags, int32_t need_x, int32_t need_w,
+                                 void *d_saved, void *d_workspace, void *d_out, void *stream);
+int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int64_t g_stride, uint32_t g_flags,
+                                  int32_t D, const void *d_saved, void *d_gx, uint32_t x_flags, void *d_gw,
+                                  uint32_t w_flags, float *d_gb, uint32_t flags, void *d_workspace,
+                                  void *stream);
+
 /* d_grad[i] *= *d_scale for i < count, unless *d_scale == 1 (then the buffer is
  * not touched: the kernel's blocks return after one load).  The counterpart of
  * `ctx.grad.mul_(loss_grad)` (transducer_loss.py:162) for a gradient that

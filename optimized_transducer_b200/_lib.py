@@ -55,6 +55,9 @@ EXPORTS = (
     "ot_b200_fp8_matmul",
     "ot_b200_joiner_logits_workspace_bytes",
     "ot_b200_joiner_logits",
+    "ot_b200_joiner_train_bytes",
+    "ot_b200_joiner_train_forward",
+    "ot_b200_joiner_train_backward",
     "ot_b200_compute_transducer_loss",
     "ot_b200_poll_errors",
     "ot_b200_read_input_status",
@@ -137,6 +140,12 @@ def load():
     lib.ot_b200_joiner_logits_workspace_bytes.argtypes = [i64, i32, i32, ctypes.POINTER(u64)]
     lib.ot_b200_joiner_logits.restype = ctypes.c_int
     lib.ot_b200_joiner_logits.argtypes = [vp, i64, i32, i64, u32, vp, i64, vp, i32, vp, u32, vp, u64, vp, vp]
+    lib.ot_b200_joiner_train_bytes.restype = ctypes.c_int
+    lib.ot_b200_joiner_train_bytes.argtypes = [i64, i32, i32, i32, i32, i32] + 3 * [ctypes.POINTER(u64)]
+    lib.ot_b200_joiner_train_forward.restype = ctypes.c_int
+    lib.ot_b200_joiner_train_forward.argtypes = [vp, i64, i32, i64, u32, vp, i32, i64, u32, vp, u32, i32, i32, vp, vp, vp, vp]
+    lib.ot_b200_joiner_train_backward.restype = ctypes.c_int
+    lib.ot_b200_joiner_train_backward.argtypes = [vp, i64, i32, i64, u32, i32, vp, vp, u32, vp, u32, vp, u32, vp, vp]
     lib.ot_b200_scale_gradient.restype = ctypes.c_int
     lib.ot_b200_scale_gradient.argtypes = [vp, i64, vp, u32, vp]
     lib.ot_b200_compute_transducer_loss.restype = ctypes.c_int

@@ -921,4 +921,108 @@ int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_
                             ws + product_off, workspace_bytes - product_off, d_out, stream);
 }
 
+// The training form's buffers, one behind the other (0 bytes where a gradient is not asked for).
+namespace {
+struct TrainLayout {
+  // kept from the forward to the backward call: W^T and X^T in blocks of 128 x 128
+  uint64_t wt = 0, wt_scale = 0, xt = 0, xt_scale = 0, saved = 0;
+  // forward scratch
+  uint64_t w = 0, w_scale = 0, x = 0, x_scale = 0, f_product = 0, forward = 0;
+  // backward scratch: the gradient of the logits along its rows and along its columns
+  uint64_t g = 0, g_scale = 0, gt = 0, gt_scale = 0, sums = 0, b_product = 0, backward = 0;
+};
+
+int train_layout(int64_t rows, int64_t D, int64_t V, int need_x, int need_w, int need_b, TrainLayout *t) {
+  uint64_t p = 0, px = 0, pw = 0;
+  int rc = ot_b200_fp8_matmul_workspace_bytes(rows, V, D, &p);
+  if (!rc && need_x) rc = ot_b200_fp8_matmul_workspace_bytes(rows, D, V, &px);
+  if (!rc && need_w) rc = ot_b200_fp8_matmul_workspace_bytes(V, D, rows, &pw);
+  if (rc) return rc;
+  const auto put = [](uint64_t *at, uint64_t *end, uint64_t bytes) {
+    *at = *end;
+    *end = (*end + bytes + 255) & ~uint64_t(255);
+  };
+  const auto blocks = [](int64_t n) { return (uint64_t)((n + kScaleBlock - 1) / kScaleBlock); };
+  put(&t->wt, &t->saved, need_x ? (uint64_t)D * row_pitch(V) : 0);
+  put(&t->wt_scale, &t->saved, need_x ? blocks(D) * blocks(V) * 4 : 0);
+  put(&t->xt, &t->saved, need_w ? (uint64_t)D * row_pitch(rows) : 0);
+  put(&t->xt_scale, &t->saved, need_w ? blocks(D) * blocks(rows) * 4 : 0);
+  put(&t->w, &t->forward, (uint64_t)V * row_pitch(D));
+  put(&t->w_scale, &t->forward, blocks(V) * blocks(D) * 4);
+  put(&t->x, &t->forward, (uint64_t)rows * row_pitch(D));
+  put(&t->x_scale, &t->forward, (uint64_t)rows * blocks(D) * 4);
+  put(&t->f_product, &t->forward, p);
+  put(&t->g, &t->backward, (uint64_t)rows * row_pitch(V));
+  put(&t->g_scale, &t->backward, (uint64_t)rows * blocks(V) * 4);
+  put(&t->gt, &t->backward, (need_w || need_b) ? (uint64_t)V * row_pitch(rows) : 0);
+  put(&t->gt_scale, &t->backward, (need_w || need_b) ? (uint64_t)V * blocks(rows) * 4 : 0);
+  put(&t->sums, &t->backward, need_b ? blocks(rows) * (uint64_t)V * 4 : 0);
+  put(&t->b_product, &t->backward, px > pw ? px : pw);
+  return OT_B200_OK;
+}
+}  // namespace
+
+int ot_b200_joiner_train_bytes(int64_t rows, int32_t D, int32_t V, int32_t need_x, int32_t need_w, int32_t need_b,
+                               uint64_t *saved_out, uint64_t *forward_out, uint64_t *backward_out) {
+  if (!saved_out || !forward_out || !backward_out)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_joiner_train_bytes: NULL output");
+  TrainLayout t;
+  const int rc = train_layout(rows, D, V, need_x, need_w, need_b, &t);
+  if (rc) return rc;
+  *saved_out = t.saved;
+  *forward_out = t.forward;
+  *backward_out = t.backward;
+  return OT_B200_OK;
+}
+
+int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags, const void *d_w,
+                                 int32_t V, int64_t w_stride, uint32_t w_flags, const float *d_bias, uint32_t out_flags,
+                                 int32_t need_x, int32_t need_w, void *d_saved, void *d_workspace, void *d_out, void *stream) {
+  TrainLayout t;
+  int rc = train_layout(rows, D, V, need_x, need_w, 0, &t);
+  if (rc) return rc;
+  if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0 ||
+      (t.saved && (!d_saved || reinterpret_cast<uintptr_t>(d_saved) % 256 != 0)))
+    return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_train_forward: a buffer is missing or not 256-byte aligned");
+  char *ws = static_cast<char *>(d_workspace), *saved = static_cast<char *>(d_saved);
+  const auto at = [](char *base, uint64_t off) { return reinterpret_cast<float *>(base + off); };
+  rc = ot_b200_fp8_quantize(d_w, V, D, w_stride, w_flags, need_x ? OT_B200_FP8_SQUARES_BOTH : OT_B200_FP8_SQUARES,
+                            ws + t.w, row_pitch(D), at(ws, t.w_scale), need_x ? saved + t.wt : nullptr,
+                            need_x ? row_pitch(V) : 0, need_x ? at(saved, t.wt_scale) : nullptr, nullptr, nullptr, stream);
+  if (!rc)
+    rc = ot_b200_fp8_quantize(d_x, rows, D, x_stride, x_flags, need_w ? OT_B200_FP8_ROWS_AND_SQUARES : OT_B200_FP8_ROWS,
+                              ws + t.x, row_pitch(D), at(ws, t.x_scale), need_w ? saved + t.xt : nullptr,
+                              need_w ? row_pitch(rows) : 0, need_w ? at(saved, t.xt_scale) : nullptr, nullptr, nullptr, stream);
+  if (!rc)
+    rc = ot_b200_fp8_matmul(ws + t.x, row_pitch(D), at(ws, t.x_scale), ws + t.w, row_pitch(D), at(ws, t.w_scale), d_bias, rows, V, D,
+                            out_flags, ws + t.f_product, t.forward - t.f_product, d_out, stream);
+  return rc;
+}
+
+int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int64_t g_stride, uint32_t g_flags, int32_t D,
+                                  const void *d_saved, void *d_gx, uint32_t x_flags, void *d_gw, uint32_t w_flags, float *d_gb,
+                                  uint32_t flags, void *d_workspace, void *stream) {
+  TrainLayout t;
+  int rc = train_layout(rows, D, V, d_gx != nullptr, d_gw != nullptr, d_gb != nullptr, &t);
+  if (rc) return rc;
+  if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0 ||
+      (t.saved && (!d_saved || reinterpret_cast<uintptr_t>(d_saved) % 256 != 0)))
+    return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_train_backward: a buffer is missing or not 256-byte aligned");
+  if (flags & ~OT_B200_REPORT_ERRORS)
+    return fail(OT_B200_ERR_ARGUMENT, "ot_b200_joiner_train_backward: flags may hold OT_B200_REPORT_ERRORS");
+  char *ws = static_cast<char *>(d_workspace), *saved = static_cast<char *>(const_cast<void *>(d_saved));
+  const auto at = [](char *base, uint64_t off) { return reinterpret_cast<float *>(base + off); };
+  const bool columns = d_gw || d_gb;
+  rc = ot_b200_fp8_quantize(d_g, rows, V, g_stride, g_flags, columns ? OT_B200_FP8_ROWS_AND_COLUMNS : OT_B200_FP8_ROWS, ws + t.g,
+                            row_pitch(V), at(ws, t.g_scale), columns ? ws + t.gt : nullptr, columns ? row_pitch(rows) : 0,
+                            columns ? at(ws, t.gt_scale) : nullptr, d_gb ? at(ws, t.sums) : nullptr, d_gb, stream);
+  if (!rc && d_gx)
+    rc = ot_b200_fp8_matmul(ws + t.g, row_pitch(V), at(ws, t.g_scale), saved + t.wt, row_pitch(V), at(saved, t.wt_scale), nullptr, rows,
+                            D, V, x_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gx, stream);
+  if (!rc && d_gw)
+    rc = ot_b200_fp8_matmul(ws + t.gt, row_pitch(rows), at(ws, t.gt_scale), saved + t.xt, row_pitch(rows), at(saved, t.xt_scale), nullptr,
+                            V, D, rows, w_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gw, stream);
+  return rc;
+}
+
 }  // extern "C"

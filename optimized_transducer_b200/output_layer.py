@@ -155,23 +155,6 @@ def _quantize(x, mode, sums=False):
     return (q, scale), ((qt, scale_t) if qt is not None else None), total
 
 
-def _matmul(a, b, m, n, k, out_dtype, bias=None):
-    """(M, N) = a (M, K) times b (N, K) transposed; a, b: (bytes, scales) pairs."""
-    dev = a[0].device
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    lib = _lib.load()
-    flags = _DTYPE_FLAG[out_dtype] | (0 if _check_mode() == "off" else _lib.REPORT_ERRORS)
-    with _on_device(dev.index):
-        need = ctypes.c_uint64()
-        _lib.check(lib.ot_b200_fp8_matmul_workspace_bytes(m, n, k, ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        _lib.check(lib.ot_b200_fp8_matmul(
-            a[0].data_ptr(), a[0].stride(0), a[1].data_ptr(), b[0].data_ptr(), b[0].stride(0), b[1].data_ptr(),
-            bias.data_ptr() if bias is not None else None, m, n, k, flags,
-            ws.data_ptr() if ws is not None else None, need.value, out.data_ptr(), _stream(dev)))
-    return out
-
-
 def quantize_weight(weight):
     """:class:`Fp8Weight` of a (V, D) float32, bfloat16 or float16 CUDA tensor: blocks
     of 128 x 128, each with the smallest power of two as its scale that keeps the
@@ -183,6 +166,18 @@ def quantize_weight(weight):
     return Fp8Weight(q.view(torch.float8_e4m3fn)[:, :weight.size(1)], scale)
 
 
+def _train_bytes(lib, *shape_and_needs):
+    """(saved, forward, backward) bytes of a training step's buffers."""
+    sizes = _WORKSPACE.get(shape_and_needs)
+    if sizes is None:
+        if len(_WORKSPACE) >= 256:
+            _WORKSPACE.clear()
+        out = [ctypes.c_uint64() for _ in range(3)]
+        _lib.check(lib.ot_b200_joiner_train_bytes(*shape_and_needs, *[ctypes.byref(n) for n in out]))
+        sizes = _WORKSPACE[shape_and_needs] = tuple(n.value for n in out)
+    return sizes
+
+
 class JoinerLogitsFunction(torch.autograd.Function):
     """See :func:`joiner_logits` (training form)."""
 
@@ -190,26 +185,46 @@ class JoinerLogitsFunction(torch.autograd.Function):
     def forward(ctx, joiner_in, weight, bias, out_dtype):
         (rows, d), v = joiner_in.shape, weight.size(0)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        # what the backward pass needs is written by the same reads, in e4m3: W^T, X^T
-        w, wt, _ = _quantize(weight.detach(), _lib.FP8_SQUARES_BOTH if need_x else _lib.FP8_SQUARES)
-        x, xt, _ = _quantize(joiner_in.detach(), _lib.FP8_ROWS_AND_SQUARES if need_w else _lib.FP8_ROWS)
-        ctx.meta = (rows, d, v, joiner_in.dtype, weight.dtype, bias.dtype if bias is not None else None)
-        ctx.save_for_backward(*(wt if need_x else (None, None)), *(xt if need_w else (None, None)))
-        return _matmul(x, w, rows, v, d, out_dtype, bias.detach() if bias is not None else None)
+        dev = joiner_in.device
+        lib = _lib.load()
+        sizes = _train_bytes(lib, rows, d, v, int(need_x), int(need_w), int(need_b))
+        report = 0 if _check_mode() == "off" else _lib.REPORT_ERRORS
+        # W^T and X^T in e4m3, all that the backward pass needs of the operands
+        saved = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
+        ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
+        out = torch.empty((rows, v), dtype=out_dtype, device=dev)
+        with _on_device(dev.index):
+            rc = lib.ot_b200_joiner_train_forward(
+                joiner_in.data_ptr(), rows, d, _row_stride(joiner_in), _DTYPE_FLAG[joiner_in.dtype], weight.data_ptr(), v,
+                _row_stride(weight), _DTYPE_FLAG[weight.dtype], bias.data_ptr() if bias is not None else None,
+                _DTYPE_FLAG[out_dtype] | report, need_x, need_w, saved.data_ptr(), ws.data_ptr(), out.data_ptr(), _stream(dev))
+        if rc:
+            _lib.check(rc)
+        ctx.meta = (rows, d, v, joiner_in.dtype, weight.dtype, sizes[2], report)
+        ctx.save_for_backward(saved)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        rows, d, v, x_dtype, w_dtype, _ = ctx.meta
+        rows, d, v, x_dtype, w_dtype, size, report = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        wt, wt_scale, xt, xt_scale = ctx.saved_tensors
-        if grad.dim() != 2 or (grad.size(1) > 1 and grad.stride(1) != 1) or (rows > 1 and grad.stride(0) < v):
+        (saved,) = ctx.saved_tensors
+        if grad.dim() != 2 or (v > 1 and grad.stride(1) != 1) or (rows > 1 and grad.stride(0) < v):
             grad = grad.contiguous()
-        both = need_w or need_b
-        g, gt, gb = _quantize(grad, _lib.FP8_ROWS_AND_COLUMNS if both else _lib.FP8_ROWS, sums=need_b)
-        gx = _matmul(g, (wt, wt_scale), rows, d, v, x_dtype) if need_x else None
-        gw = _matmul(gt, (xt, xt_scale), v, d, rows, w_dtype) if need_w else None
-        return gx, gw, gb if need_b else None, None
+        dev = grad.device
+        gx = torch.empty((rows, d), dtype=x_dtype, device=dev) if need_x else None
+        gw = torch.empty((v, d), dtype=w_dtype, device=dev) if need_w else None
+        gb = torch.empty(v, dtype=torch.float32, device=dev) if need_b else None
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        with _on_device(dev.index):
+            rc = _lib.load().ot_b200_joiner_train_backward(
+                grad.data_ptr(), rows, v, _row_stride(grad), _DTYPE_FLAG[grad.dtype], d, saved.data_ptr(),
+                gx.data_ptr() if need_x else None, _DTYPE_FLAG[x_dtype], gw.data_ptr() if need_w else None, _DTYPE_FLAG[w_dtype],
+                gb.data_ptr() if need_b else None, report, ws.data_ptr(), _stream(dev))
+        if rc:
+            _lib.check(rc)
+        return gx, gw, gb, None
 
 
 def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):

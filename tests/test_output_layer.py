@@ -34,7 +34,8 @@ def test_quantiser_argument_errors():
 
     bad = [dict(x=None), dict(rows=0), dict(cols=0), dict(rows=1 << 31), dict(ld=19), dict(flags=_lib.FP64),
            dict(flags=_lib.BF16 | _lib.FP16), dict(mode=5), dict(mode=-1), dict(q=None), dict(q=p + 8), dict(pitch=20), dict(pitch=16),
-           dict(s=None), dict(mode=_lib.FP8_SQUARES_BOTH), dict(mode=_lib.FP8_SQUARES_BOTH, qt=p, tp=32, st=p),
+           dict(s=None), dict(mode=_lib.FP8_SQUARES_BOTH), dict(mode=_lib.FP8_SQUARES_BOTH, qt=p, tp=24, st=p),
+           dict(mode=_lib.FP8_SQUARES_BOTH, qt=p, tp=144, st=p),
            dict(part=p, tot=p), dict(mode=_lib.FP8_ROWS_AND_COLUMNS, qt=p, tp=16, st=p, part=p)]
     for kw in bad:
         assert call(**kw) == _lib.ERR_ARGUMENT, kw
@@ -74,3 +75,22 @@ def test_forward_in_one_call_argument_errors():
         assert call(**kw) == _lib.ERR_WORKSPACE, kw
     for kw in (dict(x=None), dict(rows=0), dict(d=0), dict(v=0), dict(ld=19), dict(xf=_lib.FP64)):
         assert call(**kw) == _lib.ERR_ARGUMENT, kw
+
+
+def test_training_calls_argument_errors():
+    lib = _lib.load()
+    keep, p = _memory()
+    n = [ctypes.c_uint64() for _ in range(3)]
+    out = [ctypes.byref(x) for x in n]
+    assert lib.ot_b200_joiner_train_bytes(0, 20, 5, 1, 1, 1, *out) == _lib.ERR_ARGUMENT
+    assert lib.ot_b200_joiner_train_bytes(4, 20, 5, 1, 1, 1, None, *out[1:]) == _lib.ERR_ARGUMENT
+    assert lib.ot_b200_joiner_train_bytes(4, 20, 5, 0, 0, 1, *out) == _lib.OK and n[0].value == 0
+    assert lib.ot_b200_joiner_train_bytes(4, 20, 5, 1, 1, 1, *out) == _lib.OK and all(x.value for x in n)
+    fwd = lambda x=p, rows=4, ld=20, saved=p, ws=p, o=p: lib.ot_b200_joiner_train_forward(  # noqa: E731
+        x, rows, 20, ld, 0, p, 5, 20, 0, None, 0, 1, 1, saved, ws, o, None)
+    assert fwd(ws=None) == _lib.ERR_WORKSPACE and fwd(saved=p + 16) == _lib.ERR_WORKSPACE
+    assert fwd(rows=0) == _lib.ERR_ARGUMENT
+    bwd = lambda g=p, rows=4, ld=5, saved=p, flags=0, ws=p: lib.ot_b200_joiner_train_backward(  # noqa: E731
+        g, rows, 5, ld, 0, 20, saved, p, 0, p, 0, p, flags, ws, None)
+    assert bwd(ws=None) == _lib.ERR_WORKSPACE and bwd(saved=None) == _lib.ERR_WORKSPACE
+    assert bwd(g=None) == _lib.ERR_ARGUMENT and bwd(ld=4) == _lib.ERR_ARGUMENT and bwd(flags=_lib.BF16) == _lib.ERR_ARGUMENT
