@@ -297,7 +297,11 @@ constexpr int kStagedBytes = 32 * 128;           // a warp's staging tile: 32 ro
 template <int kTileN> struct Shape {
   static constexpr int columns = kTileN == 256 ? 128 : 64;
   static constexpr int epilogue_warps = 4 * kTileN / columns;
-  static constexpr int threads = 64 + 32 * epilogue_warps;
+  static constexpr int threads = 128 + 32 * epilogue_warps;  // one warpgroup for the two control warps
+  // Registers per thread of the widest tile: a launch of 384 threads gives each 168, of which the
+  // control warps need 56 at most and the epilogue's 128 sums and 64 values on their way more:
+  // 128 * 56 + 256 * 224 = 384 * 168.
+  static constexpr bool split_registers = kTileN == 256;
   static constexpr uint32_t stage_bytes = kBytesA + kTileN * kScaleBlock;
   static constexpr int ring = kTileN == 256 ? 3 : (kTileN == 128 ? 4 : 6);
   static constexpr int accumulators = kTileN == 256 ? 2 : 4;
@@ -314,24 +318,6 @@ __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(instr), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_load_16_issue(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_load_16_wait(uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.wait::ld.sync.aligned;"
-      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-      :
       : "memory");
 }
 
@@ -403,7 +389,7 @@ template <int kTileN> struct MatmulShared {
 // next block's product.
 //   warp 0   TMA producer: a (128 x 128) and b (kTileN x 128) boxes into the ring
 //   warp 1   MMA issuer
-//   others   epilogue: warp % 4 picks the TMEM lanes (rows), the rest the 64 columns
+//   warps 4..  epilogue: warp % 4 picks the TMEM lanes (rows), the rest the 64 columns
 // A wait that runs out raises the CTA's abort flag; every role leaves, the producer waits
 // (bounded) for its copies in flight, and the record of the failure goes to `sticky`.
 template <int kTileN, typename OutT>
@@ -461,6 +447,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   // The two control warps run their loops with all lanes and let one issue: stage indices,
   // barrier addresses and descriptors then live in uniform registers, where the MMAs want them.
   // (With one lane in the loop the issue of a block's MMAs took 740 cycles, more than the MMAs.)
+  if (warp < 4) {
+  if constexpr (S::split_registers) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     int s = 0;           // stage
     uint32_t phase = 1;  // parity of the wait for it; the first round finds the stages empty
@@ -524,12 +512,14 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (++buf == B) { buf = 0; free_phase ^= 1; }
       }
     }
-  } else if (warp >= 2) {
+  }
+  } else {
+    if constexpr (S::split_registers) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int quarter = warp & 3;
-    const int part = (warp - 2) >> 2;
+    const int part = (warp - 4) >> 2;
     constexpr int kCols = S::columns;
-    unsigned char *staging_tiles = staging + (size_t)(warp - 2) * S::staged_tiles * kStagedBytes;
-    float *bias_s = sh.bias[warp - 2];
+    unsigned char *staging_tiles = staging + (size_t)(warp - 4) * S::staged_tiles * kStagedBytes;
+    float *bias_s = sh.bias[warp - 4];
     uint32_t it = 0;
     bool dead = false;  // the same for all lanes: the reads of tensor memory are warp-wide
     // The scales of the next K block and the bias of the next tile are requested one block
@@ -586,20 +576,20 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                   // factors are loaded, and every block waited for that load: 460 of 1200 cycles
         asm volatile("mul.f32 %0, %1, %2;" : "=f"(s) : "f"(sa_now), "f"(sb_now));
         const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kTileN + part * kCols);
-        uint32_t r[2][16];
-        tmem_load_16_issue(taddr, r[0]);
+        uint32_t r[2][32];
+        tmem_load_32_issue(taddr, r[0]);
 #pragma unroll
-        for (int c = 0; c < kCols / 16; ++c) {
-          tmem_load_16_wait(r[c & 1]);
-          if (c + 1 < kCols / 16) {
-            tmem_load_16_issue(taddr + 16 * (c + 1), r[(c + 1) & 1]);
+        for (int c = 0; c < kCols / 32; ++c) {
+          tmem_load_32_wait(r[c & 1]);
+          if (c + 1 < kCols / 32) {
+            tmem_load_32_issue(taddr + 32 * (c + 1), r[(c + 1) & 1]);
           } else {  // the last read has landed: the accumulator goes back
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.acc_empty[buf]);
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(s, __uint_as_float(r[c & 1][i]), acc[16 * c + i]);
+          for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(s, __uint_as_float(r[c & 1][i]), acc[32 * c + i]);
         }
       }
       if (dead) break;

@@ -553,7 +553,7 @@ sample_kernel(const SampleArgs a) {
   const auto lane_of = [](int k) { return TeamT::mine(k); };  // its own inverse
   constexpr int kSteps = 16;
 
-  float least = -inf_f();  // of the logits kept so far, once a filter has asked for it
+  float least = -inf_f();  // of the logits that top-k kept
   int live = 0;
   if (top_k > 0 && top_k < a.V) {
     Pass<float> r{0.f, 0, inf_f(), 0.f};
@@ -626,7 +626,6 @@ sample_kernel(const SampleArgs a) {
   }
 
   if (top_p < 1.f) {
-    if (!(least > -inf_f())) least = least_finite();
     const S total = team.template reduce<kSum>(Pass<S>{sum_of([&](int e) { return w[e]; }), 0, 0.f, 0.f}).sum;
     const S goal = (S)top_p * total, near = (S)(2.f * a.eps) * total;
     // border: the logit with less than `goal` above it and at least that at or above it
@@ -641,8 +640,10 @@ sample_kernel(const SampleArgs a) {
     } else {
       // V logits of weight (1 - top_p) * sum / (2 V) each would not weigh what top_p leaves:
       // the border lies above them
+      // (a step down for the rounding of the sum, which may be coarse beside the temperature)
       const float floor_x = top + temperature * logf((1.f - top_p) * (float)total / (2.f * (float)a.V));
-      if (floor_x > lo) { lo = floor_x; open = true; }
+      lo = fmaxf(least, nextafterf(floor_x, -inf_f()));
+      open = lo > least;
     }
     // First by value, as far as float sums decide (their error: that of a row of 1024 at
     // most); (at_lo - above) / w(hi) is about the number of logits left between.

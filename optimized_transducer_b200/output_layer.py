@@ -39,18 +39,20 @@ def _stream(device):
     return torch.cuda.current_stream(device.index).cuda_stream
 
 
-_WORKSPACE = {}  # (rows, D, V) -> bytes: a decoder's shapes repeat from step to step
+_WORKSPACE = {}  # (device, sizes) -> bytes: the shapes of a decoder or of bucketed batches repeat
 
 
-def _workspace_bytes(lib, rows, d, v):
-    key = (rows, d, v)
+def _workspace_bytes(entry, device, *sizes):
+    """The byte counts the library's ``entry`` reports for ``sizes`` on a device, as a tuple."""
+    key = (device.index, entry, *sizes)
     n = _WORKSPACE.get(key)
     if n is None:
         if len(_WORKSPACE) >= 256:
             _WORKSPACE.clear()
-        need = ctypes.c_uint64()
-        _lib.check(lib.ot_b200_joiner_logits_workspace_bytes(rows, d, v, ctypes.byref(need)))
-        n = _WORKSPACE[key] = need.value
+        out = [ctypes.c_uint64() for _ in range(3 if entry.endswith("train_bytes") else 1)]
+        with _on_device(device.index):
+            _lib.check(getattr(_lib.load(), entry)(*sizes, *[ctypes.byref(v) for v in out]))
+        n = _WORKSPACE[key] = tuple(v.value for v in out)
     return n
 
 
@@ -59,7 +61,7 @@ def _forward(x, w, pitch, scale, bias, v, out_dtype):
     rows, d = x.shape
     dev = x.device
     lib = _lib.load()
-    size = _workspace_bytes(lib, rows, d, v)
+    (size,) = _workspace_bytes("ot_b200_joiner_logits_workspace_bytes", dev, rows, d, v)
     out = torch.empty((rows, v), dtype=out_dtype, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     flags = _DTYPE_FLAG[out_dtype] | (0 if _check_mode() == "off" else _lib.REPORT_ERRORS)
@@ -166,18 +168,6 @@ def quantize_weight(weight):
     return Fp8Weight(q.view(torch.float8_e4m3fn)[:, :weight.size(1)], scale)
 
 
-def _train_bytes(lib, *shape_and_needs):
-    """(saved, forward, backward) bytes of a training step's buffers."""
-    sizes = _WORKSPACE.get(shape_and_needs)
-    if sizes is None:
-        if len(_WORKSPACE) >= 256:
-            _WORKSPACE.clear()
-        out = [ctypes.c_uint64() for _ in range(3)]
-        _lib.check(lib.ot_b200_joiner_train_bytes(*shape_and_needs, *[ctypes.byref(n) for n in out]))
-        sizes = _WORKSPACE[shape_and_needs] = tuple(n.value for n in out)
-    return sizes
-
-
 class JoinerLogitsFunction(torch.autograd.Function):
     """See :func:`joiner_logits` (training form)."""
 
@@ -187,7 +177,7 @@ class JoinerLogitsFunction(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev = joiner_in.device
         lib = _lib.load()
-        sizes = _train_bytes(lib, rows, d, v, int(need_x), int(need_w), int(need_b))
+        sizes = _workspace_bytes("ot_b200_joiner_train_bytes", dev, rows, d, v, int(need_x), int(need_w), int(need_b))
         report = 0 if _check_mode() == "off" else _lib.REPORT_ERRORS
         # W^T and X^T in e4m3, all that the backward pass needs of the operands
         saved = torch.empty(sizes[0], dtype=torch.uint8, device=dev)

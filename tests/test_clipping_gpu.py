@@ -164,6 +164,13 @@ def test_what_overlaps_is_refused():
     assert abs(float(ot.grad_norm([g, g])) - math.sqrt(200)) <= 1e-4      # only read: allowed
 
 
+def test_nothing_to_sum():
+    empty = torch.empty(0, device=DEV)
+    assert float(ot.grad_norm([empty])) == 0.0
+    assert float(ot.clip_grad_norm_([empty, torch.empty(3, 0, device=DEV)], 1.0)) == 0.0
+    assert float(ot.grad_norm(torch.full((4,), 3.0, device=DEV))) == 6.0       # one tensor, not in a list
+
+
 def test_the_version_counter_moves():
     g = torch.ones(10, device=DEV)
     v = g._version

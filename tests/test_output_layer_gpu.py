@@ -87,7 +87,7 @@ def test_quantiser_bit_by_bit(shape, dtype):
             np.testing.assert_array_equal(as_np(qt[1]), scale if trans > 1 else scale.T)
 
 
-SHAPES = [(1, 16, 1), (1, 512, 500), (7, 100, 33), (64, 128, 128), (129, 129, 129), (300, 656, 500), (1000, 72, 1030),
+SHAPES = [(3, 1, 2), (1, 16, 1), (1, 512, 500), (7, 100, 33), (64, 128, 128), (129, 129, 129), (300, 656, 500), (1000, 72, 1030),
           (40, 1111, 2000), (2500, 512, 515)]
 
 

@@ -185,6 +185,17 @@ def test_values_at_every_magnitude():
         check(x, u, **f)
 
 
+def test_logits_whose_steps_are_coarse_beside_the_temperature():
+    """Near 1e8 neighbouring float32 numbers are 8 apart: borders fall between roundings."""
+    rng = np.random.default_rng(9)
+    for v in (400, 3000):
+        x = torch.from_numpy(1e8 + 8.0 * rng.integers(-4, 1, (20, v))).float()
+        u = torch.from_numpy(rng.random(20)).float()
+        for f in (dict(p=0.9), dict(p=0.999), dict(p=0.99, t=4.0), dict(k=5), dict(k=v // 2, p=0.99999), dict(p=0.9, t=1e-3)):
+            check(x, u, **f)
+            check(-x, u, **f)
+
+
 def test_no_rows_and_one_column():
     t, p = ot.sample_tokens(torch.empty(0, 5, device=DEV), torch.empty(0, device=DEV))
     assert t.shape == p.shape == (0,)
