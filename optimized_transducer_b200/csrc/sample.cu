@@ -49,7 +49,7 @@ struct SampleArgs {
   const int32_t *top_k;
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
-  float eps, eps_steps;
+  float eps;
   bool vec;              // four logits may be loaded at once, and V is a multiple of four
   int32_t *token;
   float *logprob;
@@ -82,15 +82,9 @@ template <typename A> struct Pass {
 // additions.  The scratch is used in two halves in turn, so one barrier per reduction will do.
 template <int kWarps, int kCtas> struct Team {
   using Sum = typename std::conditional<kWarps == 1, float, double>::type;
-  static_assert(kCtas <= kWarps, "a warp hands sums to each block");
-  // Logits that one step of a search compares with.  One inside a block, where instructions
-  // are the bound (eight: 10 700 instructions per warp and row of 5000 against 3 000); four
-  // across blocks, where a step waits for the cluster's barrier: 2.3 bits of the border per step.
-  static constexpr int kPivots = kCtas == 1 ? 1 : 4;
   struct Scratch {
     Pass<double> warp_part[2][kWarps];
     Pass<double> cta_part[2][kCtas];
-    float warp_sums[2][kWarps][kPivots], cta_sums[2][kCtas][kPivots];
     double table[16][kWarps];
     int index;
     double before, upto;
@@ -141,54 +135,6 @@ template <int kWarps, int kCtas> struct Team {
       return p.count ? __int_as_float(0x7fffffff) : p.most;
     }
     return v;
-  }
-
-  // Sums of kPivots values at once: a lane gets the sum of the value mine() names.  Each of
-  // the first steps hands half of the values to the neighbour, so the sums of four
-  // values take six exchanges and not twenty.
-  __device__ __forceinline__ static int mine(int lane) {
-    return kPivots == 4 ? ((lane & 1) << 1 | (lane & 2) >> 1) : 0;
-  }
-  __device__ __forceinline__ float sum_each(float (&v)[kPivots]) {
-    const int lane = threadIdx.x & 31;
-    int bit = 1;
-#pragma unroll
-    for (int n = kPivots; n > 1; n >>= 1, bit <<= 1) {
-      const bool upper = (lane & bit) != 0;
-#pragma unroll
-      for (int i = 0; i < n / 2; ++i) {
-        const float give = upper ? v[i] : v[i + n / 2];
-        v[i] = (upper ? v[i + n / 2] : v[i]) + __shfl_xor_sync(kFull, give, bit);
-      }
-    }
-    float t = v[0];
-#pragma unroll
-    for (int o = kPivots; o < 32; o <<= 1) t += __shfl_xor_sync(kFull, t, o);
-    if constexpr (kWarps > 1) {
-      half ^= 1;
-      if (lane < kPivots) s.warp_sums[half][threadIdx.x >> 5][lane] = t;
-      __syncthreads();
-      t = gather(s.warp_sums[half]);
-    }
-    if constexpr (kCtas > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      // the first kPivots lanes of warp c hand the block's sums to block c
-      if ((threadIdx.x >> 5) < kCtas && lane < kPivots)
-        cluster.map_shared_rank(&s.cta_sums[half][cluster.block_rank()][0], threadIdx.x >> 5)[lane] = t;
-      cluster.sync();
-      t = gather(s.cta_sums[half]);
-    }
-    return t;
-  }
-  template <int kN> __device__ __forceinline__ static float gather(const float (&part)[kN][kPivots]) {
-    const int lane = threadIdx.x & 31;
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < kN; w += 32 / kPivots)
-      if (w + lane / kPivots < kN) t += part[w + lane / kPivots][lane % kPivots];
-#pragma unroll
-    for (int o = kPivots; o < 32; o <<= 1) t += __shfl_xor_sync(kFull, t, o);
-    return t;
   }
 
   // The first element, in index order, at which the running sum of value(x, w) exceeds
@@ -380,7 +326,7 @@ __device__ __forceinline__ double exact_weight(float x, float top, double invers
 __device__ __noinline__ double exact_weight_call(float x, float top, double inverse_t) { return exact_weight(x, top, inverse_t); }
 
 template <typename T, int kWarps, int kCtas, int J, int kRowsPerBlock>
-__global__ void __launch_bounds__(kWarps * 32 * kRowsPerBlock, kWarps == 1 ? (J <= 4 ? 6 : 4) : (kWarps == 8 ? 2 : 1))
+__global__ void __launch_bounds__(kWarps * 32 * kRowsPerBlock, kWarps == 1 ? (J <= 4 ? 8 : 4) : (kWarps == 8 ? 2 : 1))
 sample_kernel(const SampleArgs a) {
   constexpr int E = 4 * J;
   using TeamT = Team<kWarps, kCtas>;
@@ -480,6 +426,17 @@ sample_kernel(const SampleArgs a) {
       return c;
     }
   };
+  const auto sum_above = [&](float border) {
+    if constexpr (kWarps == 1) {  // (one predicated addition per element, four chains)
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (x[e] > border) c[e & 3] += w[e];
+      return (c[0] + c[1]) + (c[2] + c[3]);
+    } else {
+      return sum_of([&](int e) { return x[e] > border ? w[e] : 0.f; });
+    }
+  };
   const auto least_finite = [&]() {
     Pass<float> r{0.f, 0, inf_f(), 0.f};
 #pragma unroll
@@ -543,15 +500,7 @@ sample_kernel(const SampleArgs a) {
     return m < hi && m >= lo ? m : lo;
   };
 
-  // One step of a search for a border between lo and hi: kPivots logits evenly between them,
-  // and for each what lies above it in all (weights, or counts).  A lane gets that of the
-  // pivot Team::mine() names; the sums fall from pivot to pivot, so the number of them that
-  // reach the goal says where the border is.
-  constexpr int K = TeamT::kPivots;
-  const int lane = threadIdx.x & 31;
-  const auto pivot = [&](float lo, float hi, int k) { return fminf(lo + (hi - lo) * ((float)(k + 1) / (K + 1)), hi); };
-  const auto lane_of = [](int k) { return TeamT::mine(k); };  // its own inverse
-  constexpr int kSteps = 16;
+  constexpr int kSteps = 16;  // of a search by value; the search between logits that follows ends by itself
 
   float least = -inf_f();  // of the logits that top-k kept
   int live = 0;
@@ -569,35 +518,17 @@ sample_kernel(const SampleArgs a) {
     float lo = least, hi = top, found = 0.f;  // found: a border at or above which exactly k lie
     int above = 0, at_lo = live;              // logits above hi, and at or above lo
     bool split = false;
-    const float goal = (float)top_k;          // counts stay below 2^24: exact
     bool open = false;                        // lo itself no longer counts
     for (int step = 0; step < kSteps && at_lo - above > 1 && hi - lo < 1e30f && !split; ++step) {
-      const float was_lo = lo, was_hi = hi;
-      if constexpr (K == 1) {
-        const float mid = pivot(lo, hi, 0);
-        int c[2] = {0, 0};
+      const float mid = 0.5f * lo + 0.5f * hi;
+      if (!(mid > lo && mid < hi)) break;
+      int c[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < E; ++e) c[e & 1] += x[e] > mid;
-        const int n = team.template reduce<kCount>(Pass<float>{0.f, c[0] + c[1], 0.f, 0.f}).count;
-        if (n >= top_k) { lo = mid; at_lo = n; open = true; } else { hi = mid; above = n; }
-      } else {
-        float v[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const float pk = pivot(lo, hi, k);
-          int c = 0;
-#pragma unroll
-          for (int e = 0; e < E; ++e) c += x[e] > pk;
-          v[k] = (float)c;
-        }
-        const float n = team.sum_each(v);
-        const int m = __popc(__ballot_sync(kFull, n >= goal) & ((1u << K) - 1u));
-        if (m > 0) { lo = pivot(was_lo, was_hi, m - 1); at_lo = (int)__shfl_sync(kFull, n, lane_of(m - 1)); open = true; }
-        if (m < K) { hi = pivot(was_lo, was_hi, m); above = (int)__shfl_sync(kFull, n, lane_of(m)); }
-      }
+      for (int e = 0; e < E; ++e) c[e & 1] += x[e] > mid;
+      const int n = team.template reduce<kCount>(Pass<float>{0.f, c[0] + c[1], 0.f, 0.f}).count;
+      if (n >= top_k) { lo = mid; at_lo = n; open = true; } else { hi = mid; above = n; }
       split = open && at_lo == top_k;
       found = lo;
-      if (!(lo > was_lo || hi < was_hi)) break;
     }
     if (split) {  // exactly k logits above lo
 #pragma unroll
@@ -631,7 +562,6 @@ sample_kernel(const SampleArgs a) {
     // border: the logit with less than `goal` above it and at least that at or above it
     float lo = least, hi = top;
     S above = S(0), at_lo = total;
-    bool above_is_coarse = false;  // from the first search
     bool open = false;  // lo itself no longer counts
     if (S(1) - goal > near) {
       lo = nextafterf(top, -inf_f());  // the largest alone weighs enough: nothing else is in question
@@ -645,34 +575,15 @@ sample_kernel(const SampleArgs a) {
       lo = fmaxf(least, nextafterf(floor_x, -inf_f()));
       open = lo > least;
     }
-    // First by value, as far as float sums decide (their error: that of a row of 1024 at
-    // most); (at_lo - above) / w(hi) is about the number of logits left between.
-    const float coarse = fmaxf((float)near, 2.f * a.eps_steps * (float)total);
-    for (int step = 0; step < kSteps && lo < hi && hi - lo < 1e30f && (float)(at_lo - above) > 1.5f * weight(hi); ++step) {
-      float v[K], at[K];
-#pragma unroll
-      for (int k = 0; k < K; ++k) at[k] = pivot(lo, hi, k);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (x[e] > at[k]) c[e & 3] += w[e];
-        v[k] = (c[0] + c[1]) + (c[2] + c[3]);
-      }
-      const float was_lo = lo, was_hi = hi;
-      const float n = team.sum_each(v);
-      if constexpr (K == 1) {
-        if (n >= (float)goal + coarse) { lo = at[0]; at_lo = n; open = true; }        // surely enough above it
-        else if (n <= (float)goal - coarse) { hi = at[0]; above = n; above_is_coarse = kWarps > 1; }  // surely not
-        else break;
-      } else {
-        const int m = __popc(__ballot_sync(kFull, n >= (float)goal + coarse) & ((1u << K) - 1u));
-        const int l = __popc(__ballot_sync(kFull, n > (float)goal - coarse) & ((1u << K) - 1u));
-        if (m > 0) { lo = pivot(was_lo, was_hi, m - 1); at_lo = __shfl_sync(kFull, n, lane_of(m - 1)); open = true; }
-        if (l < K) { hi = pivot(was_lo, was_hi, l); above = __shfl_sync(kFull, n, lane_of(l)); above_is_coarse = true; }
-      }
-      if (!(lo > was_lo || hi < was_hi)) break;
+    // First by value, as far as these sums decide; (at_lo - above) / w(hi) is about the number
+    // of logits left between.
+    for (int step = 0; step < kSteps && hi - lo < 1e30f && (float)(at_lo - above) > 1.5f * weight(hi); ++step) {
+      const float mid = 0.5f * lo + 0.5f * hi;
+      if (!(mid > lo && mid < hi)) break;
+      const S n = team.template reduce<kSum>(Pass<S>{sum_above(mid), 0, 0.f, 0.f}).sum;
+      if (n >= goal + near) { lo = mid; at_lo = n; open = true; }   // surely enough above it
+      else if (n <= goal - near) { hi = mid; above = n; }           // surely not
+      else break;
     }
     // Then between the logits that are left, from the least to the largest of them.
     const Pass<float> q = between(lo, hi, open);
@@ -680,7 +591,7 @@ sample_kernel(const SampleArgs a) {
     hi = q.most;
     for (int step = 0; lo < hi; ++step) {
       const float mid = middle(lo, hi, step);
-      Pass<S> s{sum_of([&](int e) { return x[e] > mid ? w[e] : 0.f; }), 0, inf_f(), -inf_f()};
+      Pass<S> s{sum_above(mid), 0, inf_f(), -inf_f()};
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         if (x[e] > mid) s.least = fminf(s.least, x[e]);
@@ -693,12 +604,11 @@ sample_kernel(const SampleArgs a) {
         const double goal64 = (double)top_p * exact_sums(mid, above64);
         enough = above64 >= goal64;
       }
-      if (enough) lo = s.least; else { hi = s.most; above = s.sum; above_is_coarse = false; }
+      if (enough) lo = s.least; else { hi = s.most; above = s.sum; }
     }
     const int equal = q.count == 1 ? 1 : equal_to(hi);
     int ties = 1;
     if (equal > 1) {
-      if (above_is_coarse) above = team.template reduce<kSum>(Pass<S>{sum_of([&](int e) { return x[e] > hi ? w[e] : 0.f; }), 0, 0.f, 0.f}).sum;
       // the i-th of the border's equals stays while above + i * w < goal
       const S wb = (S)weight(hi), n = ceil((goal - above) / wb);
       ties = (int)fmin(fmax(n, S(1)), (S)equal);
@@ -765,11 +675,9 @@ int fail(int code, const char *fmt, ...) {
 
 template <typename T, int kWarps, int kCtas, int J, int kRowsPerBlock>
 cudaError_t launch(SampleArgs a, cudaStream_t s) {
-  // additions on the longest path of a warp's row: J in a chain, 2 to join four, 5 in the warp, and u * sum;
-  // of a wide row's first search also 5 and 3 across warps and blocks
-  const float ulp = 5.9604645e-8f, ln_v = logf((float)a.V + 2.f);
-  a.eps = kWarps == 1 ? (3.f * ln_v + (J + 2 + 5 + 1) + 6) * ulp : 9.f * ulp;
-  a.eps_steps = (3.f * ln_v + (J + 2 + 5 + 5 + 3) + 8) * ulp;
+  // additions on the longest path of a warp's row: J in a chain, 2 to join four, 5 in the warp, and u * sum
+  const float ulp = 5.9604645e-8f;
+  a.eps = kWarps == 1 ? (3.f * logf((float)a.V + 2.f) + (J + 2 + 5 + 1) + 6) * ulp : 9.f * ulp;
   cudaLaunchConfig_t cfg = {};
   const int64_t blocks = kWarps == 1 ? (a.rows + kRowsPerBlock - 1) / kRowsPerBlock : a.rows * kCtas;
   if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
