@@ -196,6 +196,15 @@ def test_logits_whose_steps_are_coarse_beside_the_temperature():
             check(-x, u, **f)
 
 
+def test_weights_below_the_normal_doubles():
+    """u = 0 draws the first index of any weight at all, u = 1 the last: e^-720 still counts, e^-800 is 0."""
+    for v in (40, 2000):
+        x = torch.zeros(4, v)
+        x[0, :5], x[1, :5] = -720.0, -800.0
+        x[2, -5:], x[3, -5:] = -720.0, -800.0
+        check(x, torch.tensor([0.0, 0.0, 1.0, 1.0]))
+
+
 def test_no_rows_and_one_column():
     t, p = ot.sample_tokens(torch.empty(0, 5, device=DEV), torch.empty(0, device=DEV))
     assert t.shape == p.shape == (0,)
