@@ -182,6 +182,28 @@ def load():
     return lib
 
 
+_helper = None
+
+
+def tensors():
+    """The compiled helper of the Python layer (``csrc/tensors.cc``), bound to the library."""
+    global _helper
+    if _helper is None:
+        import torch  # noqa: F401  (its libraries have to be loaded first)
+        try:
+            from . import _tensors as helper
+        except ImportError as e:
+            raise ImportError("optimized_transducer_b200/_tensors.so is missing or does not load: build it with "
+                              f"`python -m optimized_transducer_b200.build` ({e})") from None
+        lib = load()
+        helper.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "ot_b200_last_error", "ot_b200_sample", "ot_b200_joiner_logits", "ot_b200_joiner_logits_workspace_bytes",
+            "ot_b200_joiner_train_bytes", "ot_b200_joiner_train_forward", "ot_b200_joiner_train_backward",
+            "ot_b200_clip_workspace_bytes", "ot_b200_clip_gradients")])
+        _helper = helper
+    return _helper
+
+
 def last_error():
     return load().ot_b200_last_error().decode("utf-8", "replace")
 

@@ -46,7 +46,7 @@ def start_helper():
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], cuda)], HELPER_SOURCE, "-o", HELPER,
-           f"-L{libs}", "-lc10", "-ltorch_cpu", "-ltorch_python"]
+           f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
 

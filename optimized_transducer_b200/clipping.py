@@ -4,38 +4,20 @@ backward pass of the loss and the optimizer.  The reference leaves it to
 it is two kernels for any number of tensors, of mixed types, and the clipped gradients
 may go somewhere else (the optimizer's float32 copies) instead of staying in place.
 """
-import ctypes
 import math
 
 import torch
 
 from . import _lib
-from .transducer_loss import _on_device
 
 __all__ = ["grad_norm", "clip_grad_norm_"]
 
 _KINDS = {1.0: _lib.NORM_1, 2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}
 
 
-_helper = None
-
-
-def _tensors():
-    """The compiled helper that reads a list of tensors in one call."""
-    global _helper
-    if _helper is None:
-        try:
-            from . import _tensors as helper
-        except ImportError as e:
-            raise ImportError("optimized_transducer_b200/_tensors.so is missing or does not load: build it with "
-                              f"`python -m optimized_transducer_b200.build` ({e})") from None
-        _helper = helper
-    return _helper
-
-
 def _table(tensors, who, what):
     """(pointers, counts, type flags, device) of dense CUDA tensors on one device; the first three are C arrays."""
-    pointers, counts, types, device, at, why = _tensors().describe(tensors)
+    pointers, counts, types, device, at, why = _lib.tensors().describe(tensors)
     if why == "":
         return pointers, counts, types, device
     t = tensors[at]
@@ -63,21 +45,11 @@ def _call(who, tensors, norm_type, apply, max_norm, out):
         if len(out) != len(tensors):
             raise RuntimeError(f"{who}: expected one output per gradient, got {len(out)} for {len(tensors)}")
         outs, _, out_types, out_device = _table(out, who, "the outputs")
-        at = _tensors().alike(tensors, out)
+        at = _lib.tensors().alike(tensors, out)
         if at >= 0 or out_device != device:
             raise RuntimeError(f"{who}: an output must have its gradient's shape, strides and device, got {tuple(out[at].shape)} "
                                f"on {out[at].device} for {tuple(tensors[at].shape)} on {tensors[at].device}")
-    lib = _lib.load()
-    n = len(tensors)
-    with _on_device(device):
-        need = ctypes.c_uint64()
-        _lib.check(lib.ot_b200_clip_workspace_bytes(n, ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=tensors[0].device)
-        norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-        _lib.check(lib.ot_b200_clip_gradients(
-            n, grads, counts, types, outs, out_types, kind, 1 if apply else 0, float(max_norm), ws.data_ptr(),
-            need.value, norm.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
-    return norm
+    return _lib.tensors().clip(grads, counts, types, outs, out_types, tensors[0], kind, 1 if apply else 0, float(max_norm))
 
 
 def _list(tensors):
@@ -109,5 +81,5 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
     tensors = _list(tensors)
     written = tensors if out is None else _list(out)
     norm = _call(who, tensors, norm_type, True, max_norm, None if out is None else written)
-    _tensors().written(written)
+    _lib.tensors().written(written)
     return norm

@@ -1,11 +1,21 @@
-// CPython helper of the Python layer: reads the pointers, sizes and types of a list of
-// tensors in one call.  clip_grad_norm_ is handed hundreds of tensors per step, and asking
-// each for its pointer, count, type, device and layout from Python takes about 0.3 us per
-// tensor, several times what the kernels need (600 tensors, 90 million bfloat16 elements:
-// 0.4 ms on the host, 0.1 ms on the device).  libot_b200.so itself knows nothing of torch.
+// CPython helper of the Python layer, for what costs more on the host than on the device:
+//   - reading the pointers, sizes and types of a list of tensors (clip_grad_norm_ is handed
+//     hundreds per step; asking each from Python takes about 0.3 us per property);
+//   - the usual call of an entry point with tensors that need no explanation: checks,
+//     outputs, workspace, stream and the library call in one step (joiner_logits of eight
+//     rows: 21 us through ctypes, the kernels take 8).  Whatever is not the usual case is
+//     answered with None, and the Python function then takes its own way and says what is
+//     wrong;
+//   - the autograd node of joiner_logits.
+// libot_b200.so itself knows nothing of torch; its functions come in by address (bind).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -111,9 +121,233 @@ PyObject *written(PyObject *, PyObject *list) {
   Py_RETURN_NONE;
 }
 
+// ---------------------------------------------------------------------------
+// the library's functions, by address
+// ---------------------------------------------------------------------------
+decltype(&ot_b200_last_error) f_last_error;
+decltype(&ot_b200_sample) f_sample;
+decltype(&ot_b200_joiner_logits) f_logits;
+decltype(&ot_b200_joiner_logits_workspace_bytes) f_logits_bytes;
+decltype(&ot_b200_joiner_train_bytes) f_train_bytes;
+decltype(&ot_b200_joiner_train_forward) f_train_forward;
+decltype(&ot_b200_joiner_train_backward) f_train_backward;
+decltype(&ot_b200_clip_workspace_bytes) f_clip_bytes;
+decltype(&ot_b200_clip_gradients) f_clip;
+
+// bind(addresses): in the order above.
+PyObject *bind(PyObject *, PyObject *args) {
+  unsigned long long p[9];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8)) return nullptr;
+  f_last_error = reinterpret_cast<decltype(f_last_error)>(p[0]);
+  f_sample = reinterpret_cast<decltype(f_sample)>(p[1]);
+  f_logits = reinterpret_cast<decltype(f_logits)>(p[2]);
+  f_logits_bytes = reinterpret_cast<decltype(f_logits_bytes)>(p[3]);
+  f_train_bytes = reinterpret_cast<decltype(f_train_bytes)>(p[4]);
+  f_train_forward = reinterpret_cast<decltype(f_train_forward)>(p[5]);
+  f_train_backward = reinterpret_cast<decltype(f_train_backward)>(p[6]);
+  f_clip_bytes = reinterpret_cast<decltype(f_clip_bytes)>(p[7]);
+  f_clip = reinterpret_cast<decltype(f_clip)>(p[8]);
+  Py_RETURN_NONE;
+}
+
+// A failed library call, as the Python layer raises it.
+struct LibraryError : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+void check(int rc) {
+  if (rc != OT_B200_OK) throw LibraryError(f_last_error());
+}
+
+void *stream_of(const at::Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// float32, bfloat16, float16: the flag; -1 for the rest.
+int float_flag(at::ScalarType t) { return t == at::kDouble ? -1 : type_flag(t); }
+
+bool plain_matrix(const at::Tensor &t) {
+  return t.layout() == at::kStrided && t.is_cuda() && t.dim() == 2 && t.numel() > 0 && t.is_contiguous() && float_flag(t.scalar_type()) >= 0;
+}
+
+bool plain_vector(const at::Tensor &t, at::ScalarType type, int64_t n, int device) {
+  return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+
+at::Tensor bytes_on(const at::Tensor &like, uint64_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
+
+template <typename F> PyObject *guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// sample(logits, uniforms, temperature, top_k, top_p, min_p): (tokens, logprobs) or None.
+PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (n != 6 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(args[0]), &u = THPVariable_Unpack(args[1]);
+    if (!plain_matrix(x) || x.size(1) > OT_B200_SAMPLE_MAX_V) Py_RETURN_NONE;
+    const int64_t rows = x.size(0);
+    const int device = x.get_device();
+    if (!plain_vector(u, at::kFloat, rows, device)) Py_RETURN_NONE;
+    const void *ptr[4];
+    float value[4] = {0, 0, 0, 0};
+    int k = 0;
+    for (int i = 0; i < 4; ++i) {
+      PyObject *a = args[2 + i];
+      ptr[i] = nullptr;
+      if (i == 1 && PyLong_CheckExact(a)) {
+        int overflow = 0;
+        const long long v = PyLong_AsLongLongAndOverflow(a, &overflow);
+        if (overflow || v < INT32_MIN || v > INT32_MAX) Py_RETURN_NONE;
+        k = (int)v;
+      } else if (i != 1 && PyFloat_CheckExact(a)) {
+        const double v = PyFloat_AS_DOUBLE(a);
+        if (v != v || (i == 0 && !(v >= 0.0 && v <= 1e6))) Py_RETURN_NONE;
+        value[i] = (float)v;
+      } else if (THPVariable_Check(a)) {
+        const at::Tensor &t = THPVariable_Unpack(a);
+        if (!plain_vector(t, i == 1 ? at::kInt : at::kFloat, rows, device)) Py_RETURN_NONE;
+        ptr[i] = t.data_ptr();
+      } else {
+        Py_RETURN_NONE;
+      }
+    }
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+    const auto options = x.options().requires_grad(false);
+    at::Tensor tokens = at::empty({rows}, options.dtype(at::kInt)), logprobs = at::empty({rows}, options.dtype(at::kFloat));
+    check(f_sample(x.data_ptr(), rows, (int32_t)x.size(1), x.size(1), (uint32_t)float_flag(x.scalar_type()), u.data_ptr<float>(),
+                   static_cast<const float *>(ptr[0]), value[0], static_cast<const int32_t *>(ptr[1]), k,
+                   static_cast<const float *>(ptr[2]), value[2], static_cast<const float *>(ptr[3]), value[3],
+                   tokens.data_ptr<int32_t>(), logprobs.data_ptr<float>(), stream_of(x)));
+    PyObject *a = THPVariable_Wrap(std::move(tokens)), *b = THPVariable_Wrap(std::move(logprobs));
+    PyObject *pair = PyTuple_Pack(2, a, b);
+    Py_DECREF(a);
+    Py_DECREF(b);
+    return pair;
+  });
+}
+
+// The autograd node of joiner_logits: everything the backward pass needs of the operands is
+// in one buffer, W^T and X^T in e4m3.
+struct JoinerLogits : torch::autograd::Function<JoinerLogits> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w,
+                            const std::optional<at::Tensor> &bias, int64_t out_type, int64_t report) {
+    const int64_t rows = x.size(0), d = x.size(1), v = w.size(0);
+    const bool need_x = x.requires_grad(), need_w = w.requires_grad(), need_b = bias && bias->requires_grad();
+    const c10::cuda::CUDAGuard guard(x.device());
+    uint64_t size[3];
+    check(f_train_bytes(rows, (int32_t)d, (int32_t)v, need_x, need_w, need_b, size, size + 1, size + 2));
+    at::Tensor saved = bytes_on(x, size[0]), ws = bytes_on(x, size[1]);
+    const auto type = (at::ScalarType)out_type;
+    at::Tensor out = at::empty({rows, v}, x.options().dtype(type).requires_grad(false));
+    check(f_train_forward(x.data_ptr(), rows, (int32_t)d, rows > 1 ? x.stride(0) : d, (uint32_t)float_flag(x.scalar_type()), w.data_ptr(),
+                          (int32_t)v, v > 1 ? w.stride(0) : d, (uint32_t)float_flag(w.scalar_type()), bias ? bias->data_ptr<float>() : nullptr,
+                          (uint32_t)(float_flag(type) | report), need_x, need_w, saved.data_ptr(), ws.data_ptr(), out.data_ptr(), stream_of(x)));
+    ctx->save_for_backward({saved});
+    ctx->saved_data["meta"] = std::vector<int64_t>{rows, d, v, (int64_t)x.scalar_type(), (int64_t)w.scalar_type(), need_x, need_w, need_b,
+                                                   (int64_t)size[2], report};
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "joiner_logits cannot be differentiated twice");
+    const std::vector<int64_t> m = ctx->saved_data["meta"].toIntVector();
+    const int64_t rows = m[0], d = m[1], v = m[2];
+    at::Tensor none, saved = ctx->get_saved_variables()[0], g = grads[0];
+    if (!g.defined()) return {none, none, none, none, none};
+    if ((v > 1 && g.stride(1) != 1) || (rows > 1 && g.stride(0) < v)) g = g.contiguous();
+    const c10::cuda::CUDAGuard guard(g.device());
+    const auto options = g.options().requires_grad(false);
+    at::Tensor gx, gw, gb, ws = bytes_on(g, (uint64_t)m[8]);
+    const auto x_type = (at::ScalarType)m[3], w_type = (at::ScalarType)m[4];
+    if (m[5]) gx = at::empty({rows, d}, options.dtype(x_type));
+    if (m[6]) gw = at::empty({v, d}, options.dtype(w_type));
+    if (m[7]) gb = at::empty({v}, options.dtype(at::kFloat));
+    check(f_train_backward(g.data_ptr(), rows, (int32_t)v, rows > 1 ? g.stride(0) : v, (uint32_t)float_flag(g.scalar_type()), (int32_t)d,
+                           saved.data_ptr(), gx.defined() ? gx.data_ptr() : nullptr, (uint32_t)float_flag(x_type),
+                           gw.defined() ? gw.data_ptr() : nullptr, (uint32_t)float_flag(w_type), gb.defined() ? gb.data_ptr<float>() : nullptr,
+                           (uint32_t)m[9], ws.data_ptr(), stream_of(g)));
+    return {gx, gw, gb, none, none};
+  }
+};
+
+// train(joiner_in, weight, bias or None, out dtype, report flag): the logits; arguments checked by the caller.
+PyObject *train(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 5 || !THPDtype_Check(args[3])) {
+    PyErr_SetString(PyExc_TypeError, "train: wrong arguments");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject * {
+    std::optional<at::Tensor> bias;
+    if (args[2] != Py_None) bias = THPVariable_Unpack(args[2]);
+    return THPVariable_Wrap(JoinerLogits::apply(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), bias,
+                                                (int64_t)reinterpret_cast<THPDtype *>(args[3])->scalar_type, (int64_t)PyLong_AsLong(args[4])));
+  });
+}
+
+// logits(joiner_in, weight bytes, weight scales, bias or None, out dtype, report flag): the
+// logits of a quantised weight, or None.
+PyObject *logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (n != 6 || !THPVariable_Check(args[0]) || !THPDtype_Check(args[4])) Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &scale = THPVariable_Unpack(args[2]);
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(args[4])->scalar_type;
+    if (!plain_matrix(x) || float_flag(type) < 0 || w.get_device() != x.get_device() || w.size(1) != x.size(1)) Py_RETURN_NONE;
+    const int64_t rows = x.size(0), d = x.size(1), v = w.size(0);
+    const float *bias = nullptr;
+    bool grads = x.requires_grad();
+    if (args[3] != Py_None) {
+      if (!THPVariable_Check(args[3])) Py_RETURN_NONE;
+      const at::Tensor &b = THPVariable_Unpack(args[3]);
+      if (!plain_vector(b, at::kFloat, v, x.get_device())) Py_RETURN_NONE;
+      bias = b.data_ptr<float>();
+      grads = grads || b.requires_grad();
+    }
+    if (grads && at::GradMode::is_enabled()) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(x.device());
+    uint64_t size = 0;
+    check(f_logits_bytes(rows, (int32_t)d, (int32_t)v, &size));
+    at::Tensor out = at::empty({rows, v}, x.options().dtype(type).requires_grad(false)), ws = bytes_on(x, size);
+    check(f_logits(x.data_ptr(), rows, (int32_t)d, d, (uint32_t)float_flag(x.scalar_type()), w.data_ptr(), v > 1 ? w.stride(0) : (d + 15) / 16 * 16,
+                   scale.data_ptr<float>(), (int32_t)v, bias, (uint32_t)(float_flag(type) | PyLong_AsLong(args[5])), ws.data_ptr(), size,
+                   out.data_ptr(), stream_of(x)));
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// clip(pointers, counts, types, outs or None, out types or None, first tensor, norm kind,
+// apply, max_norm): the norm; the lists come from describe().
+PyObject *clip(PyObject *, PyObject *args) {
+  const char *p, *c, *t, *o = nullptr, *ot = nullptr;
+  Py_ssize_t np, nc, nt, no, not_;
+  PyObject *like;
+  int kind, apply;
+  double max_norm;
+  if (!PyArg_ParseTuple(args, "y#y#y#z#z#Oiid", &p, &np, &c, &nc, &t, &nt, &o, &no, &ot, &not_, &like, &kind, &apply, &max_norm)) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const at::Tensor &x = THPVariable_Unpack(like);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int32_t n = (int32_t)(nc / (Py_ssize_t)sizeof(int64_t));
+    uint64_t size = 0;
+    check(f_clip_bytes(n, &size));
+    at::Tensor ws = bytes_on(x, size), norm = at::empty({}, x.options().dtype(at::kFloat).requires_grad(false));
+    check(f_clip(n, reinterpret_cast<const void *const *>(p), reinterpret_cast<const int64_t *>(c), reinterpret_cast<const int32_t *>(t),
+                 reinterpret_cast<void *const *>(o), reinterpret_cast<const int32_t *>(ot), kind, apply, max_norm, ws.data_ptr(), size,
+                 norm.data_ptr<float>(), stream_of(x)));
+    return THPVariable_Wrap(std::move(norm));
+  });
+}
+
 PyMethodDef methods[] = {{"describe", describe, METH_O, "pointers, counts and types of a list of tensors"},
                          {"alike", alike, METH_VARARGS, "whether two lists of tensors have the same shapes"},
                          {"written", written, METH_O, "moves the tensors' version counters on"},
+                         {"bind", bind, METH_VARARGS, "takes the addresses of the library's functions"},
+                         {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(sample)), METH_FASTCALL, "the usual call of sample_tokens"},
+                         {"logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(logits)), METH_FASTCALL, "the usual call of joiner_logits with a quantised weight"},
+                         {"train", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(train)), METH_FASTCALL, "joiner_logits with gradients"},
+                         {"clip", clip, METH_VARARGS, "grad_norm and clip_grad_norm_ of described tensors"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

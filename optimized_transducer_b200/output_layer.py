@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from .transducer_loss import _DTYPE_FLAG, _check_mode, _on_device
 
-__all__ = ["joiner_logits", "JoinerLogitsFunction", "Fp8Weight", "quantize_weight"]
+__all__ = ["joiner_logits", "Fp8Weight", "quantize_weight"]
 
 _BLOCK = 128
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
@@ -39,33 +39,18 @@ def _stream(device):
     return torch.cuda.current_stream(device.index).cuda_stream
 
 
-_WORKSPACE = {}  # (device, sizes) -> bytes: the shapes of a decoder or of bucketed batches repeat
-
-
-def _workspace_bytes(entry, device, *sizes):
-    """The byte counts the library's ``entry`` reports for ``sizes`` on a device, as a tuple."""
-    key = (device.index, entry, *sizes)
-    n = _WORKSPACE.get(key)
-    if n is None:
-        if len(_WORKSPACE) >= 256:
-            _WORKSPACE.clear()
-        out = [ctypes.c_uint64() for _ in range(3 if entry.endswith("train_bytes") else 1)]
-        with _on_device(device.index):
-            _lib.check(getattr(_lib.load(), entry)(*sizes, *[ctypes.byref(v) for v in out]))
-        n = _WORKSPACE[key] = tuple(v.value for v in out)
-    return n
-
-
 def _forward(x, w, pitch, scale, bias, v, out_dtype):
     """The logits of a quantised weight, (rows, V): one library call."""
     rows, d = x.shape
     dev = x.device
     lib = _lib.load()
-    (size,) = _workspace_bytes("ot_b200_joiner_logits_workspace_bytes", dev, rows, d, v)
-    out = torch.empty((rows, v), dtype=out_dtype, device=dev)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
     flags = _DTYPE_FLAG[out_dtype] | (0 if _check_mode() == "off" else _lib.REPORT_ERRORS)
     with _on_device(dev.index):
+        need = ctypes.c_uint64()
+        _lib.check(lib.ot_b200_joiner_logits_workspace_bytes(rows, d, v, ctypes.byref(need)))
+        size = need.value
+        out = torch.empty((rows, v), dtype=out_dtype, device=dev)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         rc = lib.ot_b200_joiner_logits(
             x.data_ptr(), rows, d, x.stride(0) if rows > 1 else d, _DTYPE_FLAG[x.dtype], w.data_ptr(), pitch, scale.data_ptr(), v,
             bias.data_ptr() if bias is not None else None, flags, ws.data_ptr(), size, out.data_ptr(), _stream(dev))
@@ -168,55 +153,6 @@ def quantize_weight(weight):
     return Fp8Weight(q.view(torch.float8_e4m3fn)[:, :weight.size(1)], scale)
 
 
-class JoinerLogitsFunction(torch.autograd.Function):
-    """See :func:`joiner_logits` (training form)."""
-
-    @staticmethod
-    def forward(ctx, joiner_in, weight, bias, out_dtype):
-        (rows, d), v = joiner_in.shape, weight.size(0)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = joiner_in.device
-        lib = _lib.load()
-        sizes = _workspace_bytes("ot_b200_joiner_train_bytes", dev, rows, d, v, int(need_x), int(need_w), int(need_b))
-        report = 0 if _check_mode() == "off" else _lib.REPORT_ERRORS
-        # W^T and X^T in e4m3, all that the backward pass needs of the operands
-        saved = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
-        ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
-        out = torch.empty((rows, v), dtype=out_dtype, device=dev)
-        with _on_device(dev.index):
-            rc = lib.ot_b200_joiner_train_forward(
-                joiner_in.data_ptr(), rows, d, _row_stride(joiner_in), _DTYPE_FLAG[joiner_in.dtype], weight.data_ptr(), v,
-                _row_stride(weight), _DTYPE_FLAG[weight.dtype], bias.data_ptr() if bias is not None else None,
-                _DTYPE_FLAG[out_dtype] | report, need_x, need_w, saved.data_ptr(), ws.data_ptr(), out.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc)
-        ctx.meta = (rows, d, v, joiner_in.dtype, weight.dtype, sizes[2], report)
-        ctx.save_for_backward(saved)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        rows, d, v, x_dtype, w_dtype, size, report = ctx.meta
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        (saved,) = ctx.saved_tensors
-        if grad.dim() != 2 or (v > 1 and grad.stride(1) != 1) or (rows > 1 and grad.stride(0) < v):
-            grad = grad.contiguous()
-        dev = grad.device
-        gx = torch.empty((rows, d), dtype=x_dtype, device=dev) if need_x else None
-        gw = torch.empty((v, d), dtype=w_dtype, device=dev) if need_w else None
-        gb = torch.empty(v, dtype=torch.float32, device=dev) if need_b else None
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        with _on_device(dev.index):
-            rc = _lib.load().ot_b200_joiner_train_backward(
-                grad.data_ptr(), rows, v, _row_stride(grad), _DTYPE_FLAG[grad.dtype], d, saved.data_ptr(),
-                gx.data_ptr() if need_x else None, _DTYPE_FLAG[x_dtype], gw.data_ptr() if need_w else None, _DTYPE_FLAG[w_dtype],
-                gb.data_ptr() if need_b else None, report, ws.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc)
-        return gx, gw, gb, None
-
-
 def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     """``joiner_in @ weight.T + bias`` in 8-bit floating point (e4m3), (rows, V).
 
@@ -235,20 +171,20 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     no gradient: ``joiner_in`` may then not require one."""
     who = "joiner_logits"
     served = isinstance(weight, Fp8Weight)
-    w = weight.data if served else weight
+    report = 0 if _check_mode() == "off" else _lib.REPORT_ERRORS
+    if served:
+        usual = _lib.tensors().logits(joiner_in, weight.data, weight.scale, bias, out_dtype, report)
+        if usual is not None:
+            return usual
     grads = torch.is_grad_enabled() and (joiner_in.requires_grad or (bias is not None and bias.requires_grad)
                                          or (not served and weight.requires_grad))
-    if not (served and not grads and joiner_in.is_cuda and joiner_in.is_contiguous() and joiner_in.dim() == 2
-            and joiner_in.dtype in _FLOATS and out_dtype in _FLOATS and w.device == joiner_in.device
-            and joiner_in.size(1) == w.size(1) and joiner_in.size(0) > 0
-            and (bias is None or (bias.dtype is torch.float32 and bias.dim() == 1 and bias.is_contiguous()
-                                  and bias.size(0) == w.size(0) and bias.device == joiner_in.device))):
-        _check_arguments(joiner_in, weight, bias, out_dtype, served, grads, who)
-        if joiner_in.size(0) == 0:
-            return torch.empty((0, w.size(0)), dtype=out_dtype, device=joiner_in.device)
-        if grads:
-            return JoinerLogitsFunction.apply(joiner_in, weight, bias, out_dtype)
+    _check_arguments(joiner_in, weight, bias, out_dtype, served, grads, who)
+    if joiner_in.size(0) == 0:
+        return torch.empty((0, weight.shape[0]), dtype=out_dtype, device=joiner_in.device)
+    if grads:
+        return _lib.tensors().train(joiner_in, weight, bias, out_dtype, report)
     if served:
+        w = weight.data
         return _forward(joiner_in, w, w.stride(0) if w.size(0) > 1 else _pitch(w.size(1)), weight.scale, bias, w.size(0), out_dtype)
     q, scale = _quantize(weight, _lib.FP8_SQUARES)[0]
     return _forward(joiner_in, q, q.size(1), scale, bias, weight.size(0), out_dtype)

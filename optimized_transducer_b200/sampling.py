@@ -45,16 +45,14 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     without a finite maximum (everything ``-inf``, or a NaN or ``+inf`` in it), or whose
     own settings are out of range (``uniforms`` outside [0, 1], ``temperature`` outside
     [0, 1e6], a NaN), gets token -1 and log-probability NaN."""
-    t_ptr, t = (None, temperature) if type(temperature) is float else _setting(temperature, "temperature", torch.float32, logits)
-    k_ptr, k = (None, top_k) if type(top_k) is int else _setting(top_k, "top_k", torch.int32, logits)
-    p_ptr, p = (None, top_p) if type(top_p) is float else _setting(top_p, "top_p", torch.float32, logits)
-    m_ptr, m = (None, min_p) if type(min_p) is float else _setting(min_p, "min_p", torch.float32, logits)
-    if not (logits.is_cuda and logits.dtype in _FLOATS and logits.dim() == 2 and logits.is_contiguous()
-            and 1 <= logits.size(1) <= MAX_V and logits.size(0) > 0 and uniforms.dtype is torch.float32
-            and uniforms.is_contiguous() and uniforms.dim() == 1 and uniforms.size(0) == logits.size(0)
-            and uniforms.device == logits.device and (t_ptr is not None or 0.0 <= t <= 1e6) and p == p and m == m
-            and -0x80000000 <= k <= 0x7fffffff):
-        _check_arguments(logits, uniforms, t_ptr, t, k, p, m)
+    usual = _lib.tensors().sample(logits, uniforms, temperature, top_k, top_p, min_p)
+    if usual is not None:
+        return usual
+    t_ptr, t = _setting(temperature, "temperature", torch.float32, logits)
+    k_ptr, k = _setting(top_k, "top_k", torch.int32, logits)
+    p_ptr, p = _setting(top_p, "top_p", torch.float32, logits)
+    m_ptr, m = _setting(min_p, "min_p", torch.float32, logits)
+    _check_arguments(logits, uniforms, t_ptr, t, k, p, m)
     rows, v = logits.shape
     device = logits.device
     tokens = torch.empty(rows, dtype=torch.int32, device=device)

@@ -206,6 +206,35 @@ def test_gradients_of_some_operands_only():
     assert torch.equal(bb.grad, torch.full_like(bb, 32.0))
 
 
+def test_a_second_derivative_is_refused():
+    x = torch.randn(4, 16, device=DEV, requires_grad=True)
+    y = ot.joiner_logits(x, torch.randn(3, 16, device=DEV), out_dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_calls_that_are_not_the_usual_one_give_the_same():
+    """Strided operands and int settings take another way through the Python layer."""
+    x = torch.randn(20, 64, device=DEV)
+    w = ot.quantize_weight(torch.randn(33, 64, device=DEV))
+    b = torch.randn(33, device=DEV)
+    wide = torch.zeros(20, 80, device=DEV)
+    wide[:, :64] = x
+    assert torch.equal(ot.joiner_logits(wide[:, :64], w, b), ot.joiner_logits(x, w, b))
+    assert torch.equal(ot.joiner_logits(x.requires_grad_(True).detach(), w, b), ot.joiner_logits(x.detach(), w, b))
+    with pytest.raises(RuntimeError, match="inference"):
+        ot.joiner_logits(x, w, b)
+    with torch.no_grad():
+        assert not ot.joiner_logits(x, w, b).requires_grad
+    for bad in (b[:5], b.double(), b.cpu(), torch.stack([b, b], 1)[:, 0]):
+        with pytest.raises(RuntimeError, match="bias"):
+            ot.joiner_logits(x.detach(), w, bad)
+    with pytest.raises(RuntimeError, match="out_dtype"):
+        ot.joiner_logits(x.detach(), w, b, out_dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="joiner_in"):
+        ot.joiner_logits(x.detach()[:, :63], w, b)
+
+
 def test_what_is_not_finite_stays_in_its_block():
     rng = np.random.default_rng(9)
     x = torch.from_numpy(rng.standard_normal((6, 300))).float().to(DEV)

@@ -205,6 +205,24 @@ def test_weights_below_the_normal_doubles():
         check(x, torch.tensor([0.0, 0.0, 1.0, 1.0]))
 
 
+def test_refusals_on_the_gpu():
+    x, u = torch.randn(4, 50, device=DEV), torch.rand(4, device=DEV)
+    want = ot.sample_tokens(x, u, temperature=1.0, top_k=3)
+    got = ot.sample_tokens(x, u, temperature=1, top_k=True * 3, top_p=1, min_p=0)     # ints where floats are usual
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for kw, what in ((dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+                     (dict(top_p=float("nan")), "top_p"), (dict(top_k=1 << 40), "top_k"), (dict(min_p=u[:2]), "min_p"),
+                     (dict(top_k=u), "top_k"), (dict(temperature=u.cpu()), "temperature")):
+        with pytest.raises(RuntimeError, match=what):
+            ot.sample_tokens(x, u, **kw)
+    for bad in (u[:3], u.double(), u.cpu(), torch.stack([u, u], 1)[:, 0]):
+        with pytest.raises(RuntimeError, match="uniforms"):
+            ot.sample_tokens(x, bad)
+    for bad in (x.double(), x[:, ::2], x[0], torch.empty(2, 0, device=DEV), torch.empty(1, 262145, device=DEV)):
+        with pytest.raises(RuntimeError, match="logits"):
+            ot.sample_tokens(bad, u)
+
+
 def test_no_rows_and_one_column():
     t, p = ot.sample_tokens(torch.empty(0, 5, device=DEV), torch.empty(0, device=DEV))
     assert t.shape == p.shape == (0,)
