@@ -95,6 +95,11 @@ template <typename T> struct Quad {
     t[j] = x;
     memcpy(&raw, t, sizeof(raw));
   }
+  // Makes the compiler forget what it converted so far: in 16 bits converting again costs an
+  // instruction, keeping 64 floats alive from one pass over the tile to the next costs spills.
+  __device__ __forceinline__ void forget() {
+    if constexpr (sizeof(T) == 2) asm volatile("" : "+r"(raw.x), "+r"(raw.y));
+  }
   __device__ __forceinline__ float at(int j) const {
     T t[4];
     memcpy(t, &raw, sizeof(raw));
@@ -110,6 +115,28 @@ template <typename T> struct Quad {
       memcpy(w, &raw, 8);
       const uint32_t m = __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
       return widen(max(m & 0xffffu, m >> 16));
+    }
+  }
+  // ... and of the largest of each of the four columns of a lane's rows.
+  __device__ __forceinline__ static void column_tops(const Quad (&v)[kQuantRows], uint32_t (&top)[4]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        top[j] = 0u;
+#pragma unroll
+        for (int i = 0; i < kQuantRows; ++i) top[j] = max(top[j], abs_bits(v[i].at(j)));
+      }
+    } else {
+      uint32_t m[2] = {0u, 0u};
+#pragma unroll
+      for (int i = 0; i < kQuantRows; ++i) {
+        uint32_t w[2];
+        memcpy(w, &v[i].raw, 8);
+        m[0] = __vmaxu2(m[0], w[0] & 0x7fff7fffu);
+        m[1] = __vmaxu2(m[1], w[1] & 0x7fff7fffu);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top[j] = widen((j & 1) ? m[j >> 1] >> 16 : m[j >> 1] & 0xffffu);
     }
   }
   // Float bits of |x| from the bits of the element type's |x|.
@@ -133,9 +160,9 @@ template <typename T> struct Quad {
 template <typename T, int kPlain, int kTrans, bool kSums>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 3 : 2)
 quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
-  __shared__ uint32_t top_s[8][kScaleBlock];   // column maxima of each warp (or one word per warp)
-  __shared__ float sum_s[kSums ? 8 : 1][kScaleBlock];
-  __shared__ float inv_s[kScaleBlock];
+  __shared__ __align__(16) uint32_t top_s[8][kScaleBlock];   // column maxima of each warp (or one word per warp)
+  __shared__ __align__(16) float sum_s[kSums ? 8 : 1][kScaleBlock];
+  __shared__ __align__(16) float inv_s[kScaleBlock];
   __shared__ __align__(16) uint8_t tile_s[kTrans != kNone ? kScaleBlock * kScaleBlock : 16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rt = blockIdx.x / (uint32_t)a.col_tiles;
@@ -166,18 +193,25 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
   }
 
   if constexpr (kPlain == kRowBlocks) {
-    float mine = 0.f;
-    uint8_t *q = a.q + row0 * a.q_pitch + col;
+    // every lane learns every row's maximum, lane i works out the scale of row i
+    uint32_t my_top = 0u;
 #pragma unroll
     for (int i = 0; i < kQuantRows; ++i) {
       const uint32_t top = __reduce_max_sync(kFull, v[i].top());
-      float inv;
-      const float s = block_scale(top, inv);
-      if (lane == i) mine = s;
-      if (i < rows_here && col < a.cols)  // the pitch is a multiple of 16: the word stays inside the row
-        *reinterpret_cast<uint32_t *>(q + i * a.q_pitch) = pack4(v[i].at(0) * inv, v[i].at(1) * inv, v[i].at(2) * inv, v[i].at(3) * inv);
+      if (lane == i) my_top = top;
     }
-    if (lane < rows_here) a.scale[(int64_t)ct * a.rows + row0 + lane] = mine;
+    float my_inv;
+    const float my_scale = block_scale(my_top, my_inv);
+    if (lane < rows_here) a.scale[(int64_t)ct * a.rows + row0 + lane] = my_scale;
+    uint8_t *q = a.q + row0 * a.q_pitch + col;
+    const int rows_stored = col < a.cols ? rows_here : 0;  // the pitch is a multiple of 16: a word stays inside its row
+#pragma unroll
+    for (int i = 0; i < kQuantRows; ++i) {
+      const float inv = __shfl_sync(kFull, my_inv, i);
+      const uint32_t word = pack4(v[i].at(0) * inv, v[i].at(1) * inv, v[i].at(2) * inv, v[i].at(3) * inv);
+      if (i < rows_stored) *reinterpret_cast<uint32_t *>(q) = word;
+      q += a.q_pitch;
+    }
   }
   float square_inv = 0.f;
   if constexpr (kPlain == kSquareBlocks || kTrans == kSquareBlocks) {
@@ -204,19 +238,21 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
               pack4(v[i].at(0) * square_inv, v[i].at(1) * square_inv, v[i].at(2) * square_inv, v[i].at(3) * square_inv);
     }
   }
+#pragma unroll
+  for (int i = 0; i < kQuantRows; ++i) v[i].forget();
   if constexpr (kTrans == kColumnBlocks || kSums) {
+    if constexpr (kTrans == kColumnBlocks) {
+      uint32_t top[4];
+      Quad<T>::column_tops(v, top);
+      *reinterpret_cast<uint4 *>(&top_s[warp][4 * lane]) = make_uint4(top[0], top[1], top[2], top[3]);
+    }
+    if constexpr (kSums) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t top = 0u;
-      float sum = 0.f;
+      for (int i = 0; i < kQuantRows; ++i)
 #pragma unroll
-      for (int i = 0; i < kQuantRows; ++i) {
-        const float f = v[i].at(j);
-        top = max(top, abs_bits(f));
-        sum += f;
-      }
-      if (kTrans == kColumnBlocks) top_s[warp][4 * lane + j] = top;
-      if (kSums) sum_s[warp][4 * lane + j] = sum;
+        for (int j = 0; j < 4; ++j) sum[j] += v[i].at(j);
+      *reinterpret_cast<float4 *>(&sum_s[warp][4 * lane]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
     }
     __syncthreads();
     if (threadIdx.x < kScaleBlock) {
@@ -244,8 +280,12 @@ quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
     // 16-byte pieces of a column are permuted by the column's group of four, so that the
     // eight lanes of a store phase (columns four apart) hit different banks.
 #pragma unroll
+    for (int i = 0; i < kQuantRows; ++i) v[i].forget();
+    __align__(16) float inv_of[4] = {square_inv, square_inv, square_inv, square_inv};
+    if (kTrans == kColumnBlocks) *reinterpret_cast<float4 *>(inv_of) = *reinterpret_cast<const float4 *>(inv_s + 4 * lane);
+#pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float inv = kTrans == kSquareBlocks ? square_inv : inv_s[4 * lane + j];
+      const float inv = inv_of[j];
       uint32_t w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
