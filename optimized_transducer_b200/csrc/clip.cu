@@ -12,7 +12,8 @@
 // sum depends on the order in which blocks run, and when the factor is 1 and the gradients
 // stay where they are apply_kernel ends there.  Bound by HBM: one read for the norm, one
 // read (from L2 what still is there: it runs over the tensors backwards) and one write for
-// the clipping.
+// the clipping.  400 M float gradients into other buffers: 0.81 ms for 4.8 GB, 5.9 TB/s; 90 M
+// bfloat16 in 600 tensors into float buffers: 0.14 ms.
 //
 // The tensors' pointers travel as kernel arguments, so a call copies nothing to the device
 // and a captured call replays with the pointers it was captured with.

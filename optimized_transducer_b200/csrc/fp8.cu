@@ -155,8 +155,11 @@ template <typename T> struct Quad {
 // One block per 128 x 128 tile of x; a warp holds 16 rows, a lane four columns of each, in
 // registers and in the type they have (half the registers in 16 bits: three blocks per SM
 // instead of one), so the tile is read once whatever is written: bytes along the rows
-// (kPlain), transposed bytes (kTrans), and the tile's column sums.  Bound by HBM: sizeof(T)
-// bytes read and one or two written per element.
+// (kPlain), transposed bytes (kTrans), and the tile's column sums.  Bound by HBM (sizeof(T)
+// bytes read and one or two written per element) and, with everything asked for, by
+// instruction issue: 116 250 x 512 bfloat16 along the rows 34 us = 5.3 TB/s; 116 250 x 5000 along
+// rows and columns with sums 496 us = 4.7 TB/s (26 instructions per element with every lane
+// working out every row's scale and float column maxima: 583 us).
 template <typename T, int kPlain, int kTrans, bool kSums>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 3 : 2)
 quantize_kernel(const T *__restrict__ x, const QuantArgs a) {
@@ -430,6 +433,10 @@ template <int kTileN> struct MatmulShared {
 //   warp 0   TMA producer: a (128 x 128) and b (kTileN x 128) boxes into the ring
 //   warp 1   MMA issuer
 //   warps 4..  epilogue: warp % 4 picks the TMEM lanes (rows), the rest the 64 columns
+// Measured (116 250 rows): logits from D = 512 to V = 5000 470-510 us, dX (V -> D) 350 us =
+// 1.7 PFLOP/s, dW 373 us.  A K block takes about 0.6 us whichever of the copies, the MMAs, the
+// reads or the multiply-adds is left out: with two accumulators the round trip between the
+// MMA warp and the epilogue sets the pace, not one of the pipes.
 // A wait that runs out raises the CTA's abort flag; every role leaves, the producer waits
 // (bounded) for its copies in flight, and the record of the failure goes to `sticky`.
 template <int kTileN, typename OutT>

@@ -20,7 +20,7 @@
 // In wider rows more sums come close to each other: there the argument is carried in two
 // floats and sums of four weights are added in double, so eps = 9 * 2^-24.  A
 // comparison of two such sums that is closer than twice that is made again with double sums
-// (about one row in a hundred at 500 symbols).  Nothing is sorted: a filter's border is a
+// (few rows at 500 symbols, most at 100 000).  Nothing is sorted: a filter's border is a
 // logit, found by bisection on the values and then between the logits that are still in
 // question.
 #include <cooperative_groups.h>
@@ -328,8 +328,8 @@ __device__ __noinline__ double exact_weight_call(float x, float top, double inve
 
 // A row lives in the registers of its threads, 4 J logits and their weights in each, so HBM is
 // read once; what bounds the kernel is the work on a row.  80 000 rows of 500 (float, 160 MB):
-// 53 us without a filter, 157 us with top-p (about 1 500 instructions per row; the issue slots
-// are 72 % used), 24 us would be the read.  A few rows are bound by the chain of a search's
+// 53 us without a filter, 157 us with top-p (about 1 900 instructions per row; the issue slots
+// are 85 % used), 24 us would be the read.  A few rows are bound by the chain of a search's
 // steps (a comparison per logit, then a reduction: 350 cycles in a warp, 600 in a block, 1.5 us
 // in a cluster): 256 x 5000 with all filters 26 us, 16 x 100003 with top-p and min-p 52 us.
 // Tried and slower: four or eight pivots per step (the instructions grow faster than the
@@ -580,8 +580,8 @@ sample_kernel(const SampleArgs a) {
       open = true;
     } else {
       // V logits of weight (1 - top_p) * sum / (2 V) each would not weigh what top_p leaves:
-      // the border lies above them
-      // (a step down for the rounding of the sum, which may be coarse beside the temperature)
+      // the border lies above them (and a step down, for the rounding of this sum, which may be
+      // coarse beside the temperature)
       const float floor_x = top + temperature * logf((1.f - top_p) * (float)total / (2.f * (float)a.V));
       lo = fmaxf(least, nextafterf(floor_x, -inf_f()));
       open = lo > least;

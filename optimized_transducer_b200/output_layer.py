@@ -167,7 +167,8 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     ``d weight = q(G^T) q(X)`` in e4m3 (the gradient G of the logits in blocks of 128
     along the contraction, X in blocks of 128 x 128), ``d bias`` the float32 column
     sums of G.  X and W are kept for the backward pass in e4m3 (one byte per element),
-    so overwriting ``joiner_in`` afterwards does no harm.  An :class:`Fp8Weight` has
+    so overwriting ``joiner_in`` afterwards does no harm.  The gradient is not itself
+    differentiable (``create_graph=True`` is refused).  An :class:`Fp8Weight` has
     no gradient: ``joiner_in`` may then not require one."""
     who = "joiner_logits"
     served = isinstance(weight, Fp8Weight)
