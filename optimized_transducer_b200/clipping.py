@@ -73,13 +73,18 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
     ``transducer_loss_and_grad`` returns.  They are scaled in place (left untouched when
     the factor is 1), or, with ``out`` (one tensor per gradient, same shape and strides,
     any of the types), written there and left as they are.  No two tensors may overlap.
-    The host does not wait for the device.  As in torch an infinite norm scales by 0 and
+    Tensors that require a gradient are refused: unlike torch's function this one is not
+    given the parameters.  The host does not wait for the device.  As in torch an infinite norm scales by 0 and
     a NaN one by NaN."""
     who = "clip_grad_norm_"
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"{who}: max_norm must not be negative or a NaN, got {max_norm}")
     tensors = _list(tensors)
     written = tensors if out is None else _list(out)
+    at = _lib.tensors().writable(written)
+    if at >= 0:
+        raise RuntimeError(f"{who}: tensor {at} requires a gradient: pass the gradients (p.grad), not the parameters, and no "
+                           "gradient that is part of a graph")
     norm = _call(who, tensors, norm_type, True, max_norm, None if out is None else written)
     _lib.tensors().written(written)
     return norm

@@ -103,6 +103,18 @@ PyObject *alike(PyObject *, PyObject *args) {
   }
 }
 
+// writable(list): the index of the first tensor that autograd follows (a parameter, or a
+// gradient that is part of a graph), -1 when there is none.
+PyObject *writable(PyObject *, PyObject *list) {
+  PyObject *seq = PySequence_Fast(list, "expected a sequence of tensors");
+  if (seq == nullptr) return nullptr;
+  Py_ssize_t found = -1;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq) && found < 0; ++i)
+    if (THPVariable_Check(PySequence_Fast_GET_ITEM(seq, i)) && THPVariable_Unpack(PySequence_Fast_GET_ITEM(seq, i)).requires_grad()) found = i;
+  Py_DECREF(seq);
+  return PyLong_FromSsize_t(found);
+}
+
 // written(list): the tensors' version counters move on, as after any write that autograd
 // has to know of (inference tensors have none).
 PyObject *written(PyObject *, PyObject *list) {
@@ -342,6 +354,7 @@ PyObject *clip(PyObject *, PyObject *args) {
 
 PyMethodDef methods[] = {{"describe", describe, METH_O, "pointers, counts and types of a list of tensors"},
                          {"alike", alike, METH_VARARGS, "whether two lists of tensors have the same shapes"},
+                         {"writable", writable, METH_O, "the first tensor that requires a gradient"},
                          {"written", written, METH_O, "moves the tensors' version counters on"},
                          {"bind", bind, METH_VARARGS, "takes the addresses of the library's functions"},
                          {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(sample)), METH_FASTCALL, "the usual call of sample_tokens"},

@@ -46,3 +46,11 @@ def test_argument_errors():
         assert "ot_b200_clip_gradients" in _lib.last_error()
     for kw in (dict(ws=None), dict(wb=need.value - 1), dict(ws=p + 516)):
         assert call(**kw) == _lib.ERR_WORKSPACE, kw
+
+
+def test_parameters_in_place_of_their_gradients_are_refused():
+    p = torch.nn.Parameter(torch.ones(3))
+    with pytest.raises(RuntimeError, match="not the parameters"):
+        ot.clip_grad_norm_([torch.ones(3), p], 1.0)
+    with pytest.raises(RuntimeError, match="not the parameters"):
+        ot.clip_grad_norm_([torch.ones(3)], 1.0, out=[p])
