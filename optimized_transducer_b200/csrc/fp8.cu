@@ -419,6 +419,7 @@ template <int kTileN> struct MatmulShared {
   uint64_t empty[Shape<kTileN>::ring];         // MMA -> TMA
   uint64_t acc_full[Shape<kTileN>::accumulators];   // MMA -> epilogue: one K block's product is complete
   uint64_t acc_empty[Shape<kTileN>::accumulators];  // epilogue -> MMA, one arrival per warp: 256 of them took as long as the block's MMAs
+  uint64_t drained;                            // every MMA issued so far has completed (after an abort)
   uint32_t tmem_base;
   int never;
   volatile int abort;
@@ -432,13 +433,14 @@ template <int kTileN> struct MatmulShared {
 // next block's product.
 //   warp 0   TMA producer: a (128 x 128) and b (kTileN x 128) boxes into the ring
 //   warp 1   MMA issuer
-//   warps 4..  epilogue: warp % 4 picks the TMEM lanes (rows), the rest the 64 columns
+//   warps 4..  epilogue: warp % 4 picks the TMEM lanes (rows), the rest the columns
 // Measured (116 250 rows): logits from D = 512 to V = 5000 470-510 us, dX (V -> D) 350 us =
-// 1.7 PFLOP/s, dW 373 us.  A K block takes about 0.6 us whichever of the copies, the MMAs, the
-// reads or the multiply-adds is left out: with two accumulators the round trip between the
-// MMA warp and the epilogue sets the pace, not one of the pipes.
+// 1.7 PFLOP/s, dW 373 us.  A K block takes about 1 150 cycles, of which the epilogue is busy for
+// 990, and the SMs' clock falls to 1.5 - 1.7 GHz under this load; sixteen epilogue warps of 64
+// columns, a leaner wait and other depths of the reads all came out within 3 % of this form.
 // A wait that runs out raises the CTA's abort flag; every role leaves, the producer waits
-// (bounded) for its copies in flight, and the record of the failure goes to `sticky`.
+// (bounded) for its copies in flight and the issuer for its MMAs, and the record of the
+// failure goes to `sticky`.
 template <int kTileN, typename OutT>
 __global__ void __launch_bounds__(Shape<kTileN>::threads, 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -454,6 +456,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   if (threadIdx.x == 0) {
     for (int i = 0; i < R; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
     for (int i = 0; i < B; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], S::epilogue_warps); }
+    mbar_init(&sh.drained, 1);
     sh.abort = 0;
     sh.never = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -558,6 +561,11 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (++s == R) { s = 0; full_phase ^= 1; }
         if (++buf == B) { buf = 0; free_phase ^= 1; }
       }
+    }
+    if (dead && blocks > 0) {  // the MMAs in flight still read shared memory and write tensor memory
+      if (elect_one()) mma_commit(&sh.drained);
+      __syncwarp();
+      mbar_wait(&sh.drained, 0, &sh.never);
     }
   }
   } else {
