@@ -104,11 +104,23 @@ template <int kWarps, int kCtas> struct Team {
     }
     return p;
   }
-  template <typename A, int kN> __device__ __forceinline__ static Pass<A> entry(const Pass<double> (&part)[kN]) {
+  // The same over kN entries (a power of two) that a reduction has left in shared memory.
+  // Lane l takes entry l modulo kN, so a sum needs log2(kN) exchanges and every lane has it.
+  template <int kWhat, typename A, int kN> __device__ __forceinline__ static Pass<A> over(const Pass<double> (&part)[kN]) {
     const int lane = threadIdx.x & 31;
-    if (lane >= kN) return Pass<A>{A(0), 0, inf_f(), -inf_f()};
-    const Pass<double> &t = part[lane];
-    return Pass<A>{(A)t.sum, t.count, t.least, t.most};
+    const Pass<double> &t = part[lane % kN];
+    Pass<A> p{A(0), 0, 0.f, 0.f};
+    if (kWhat & kSum) {
+      p.sum = (A)t.sum;
+#pragma unroll
+      for (int o = kN / 2; o > 0; o >>= 1) p.sum += __shfl_xor_sync(kFull, p.sum, o);
+    }
+    if (kWhat & kCount) p.count = __reduce_add_sync(kFull, lane < kN ? t.count : 0);
+    if (kWhat & kEnds) {
+      p.least = warp_min_f(t.least);
+      p.most = warp_max_f(t.most);
+    }
+    return p;
   }
   template <int kWhat, typename A> __device__ __forceinline__ Pass<A> reduce(Pass<A> p) {
     p = across<kWhat>(p);
@@ -116,14 +128,14 @@ template <int kWarps, int kCtas> struct Team {
       half ^= 1;
       if ((threadIdx.x & 31) == 0) s.warp_part[half][threadIdx.x >> 5] = Pass<double>{(double)p.sum, p.count, p.least, p.most};
       __syncthreads();
-      p = across<kWhat>(entry<A>(s.warp_part[half]));
+      p = over<kWhat, A>(s.warp_part[half]);
     }
     if constexpr (kCtas > 1) {
       cg::cluster_group cluster = cg::this_cluster();
       if (threadIdx.x < kCtas)
         *cluster.map_shared_rank(&s.cta_part[half][cluster.block_rank()], threadIdx.x) = Pass<double>{(double)p.sum, p.count, p.least, p.most};
       cluster.sync();
-      p = across<kWhat>(entry<A>(s.cta_part[half]));
+      p = over<kWhat, A>(s.cta_part[half]);
     }
     return p;
   }
