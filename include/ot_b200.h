@@ -336,7 +336,8 @@ int ot_b200_fp8_quantize(const void *d_x, int64_t rows, int32_t cols, int64_t ro
  * d_bias (N) float or NULL.  When K is long and M x N small the work is split along K
  * and the pieces' sums are joined in a fixed order: the workspace (16-byte aligned) holds
  * them, 0 bytes otherwise.  `flags` may hold OT_B200_REPORT_ERRORS: a wait of the kernel
- * that ran out (never in normal operation) is then recorded for the next call. */
+ * that ran out (never in normal operation) is then recorded for the next call.  The tiles
+ * of the block whose wait it was hold NaN, recorded or not. */
 int ot_b200_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, uint64_t *bytes_out);
 int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a, const void *d_b,
                        int64_t b_pitch, const float *d_scale_b, const float *d_bias, int64_t M,

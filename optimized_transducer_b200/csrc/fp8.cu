@@ -21,6 +21,7 @@
 #include <cuda_fp8.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
@@ -405,6 +406,7 @@ struct MatmulArgs {
   int unit;             // bytes per store, the largest of 8, 4, 2 that divides the rows' pitch and the base; 0: TMA stores (16 bytes do)
   int32_t *sticky;      // error record, or NULL
   int32_t seq;
+  int wait_limit;       // polls of a barrier before a wait gives up
 };
 
 // True for one lane of a converged warp.
@@ -412,6 +414,13 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
   return yes != 0;
+}
+
+// Where the roles of a CTA meet, each at the end of its own branch.
+__device__ __forceinline__ void meet_in_cta() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  asm volatile("bar.sync 0;" ::: "memory");
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
 template <int kTileN> struct MatmulShared {
@@ -422,7 +431,7 @@ template <int kTileN> struct MatmulShared {
   uint64_t drained;                            // every MMA issued so far has completed (after an abort)
   uint32_t tmem_base;
   int never;
-  volatile int abort;
+  volatile int abort;                          // a wait ran out: every role leaves its loop
   alignas(16) float bias[Shape<kTileN>::epilogue_warps][Shape<kTileN>::columns];  // read as float4
 };
 
@@ -438,9 +447,12 @@ template <int kTileN> struct MatmulShared {
 // 1.7 PFLOP/s, dW 373 us.  A K block takes about 1 150 cycles, of which the epilogue is busy for
 // 990, and the SMs' clock falls to 1.5 - 1.7 GHz under this load; sixteen epilogue warps of 64
 // columns, a leaner wait and other depths of the reads all came out within 3 % of this form.
-// A wait that runs out raises the CTA's abort flag; every role leaves, the producer waits
-// (bounded) for its copies in flight and the issuer for its MMAs, and the record of the
-// failure goes to `sticky`.
+// A wait that runs out raises the CTA's abort flag and every role leaves its loop.  Whichever
+// role that was, and however far the others had come (the producer runs a ring ahead, and
+// leaves without a wait when its K blocks fit the ring), they all look at the flag once more
+// behind the barrier where they meet: the producer then waits (bounded) for its copies in
+// flight and writes the record of the failure to `sticky`, the issuer waits for its MMAs in
+// flight, and the epilogue fills the CTA's tiles with NaN.
 template <int kTileN, typename OutT>
 __global__ void __launch_bounds__(Shape<kTileN>::threads, 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -508,7 +520,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const Place p = place(tile);
       for (int kb = p.k0; kb < p.k1; ++kb) {
         if (issued >= (uint32_t)R) {
-          dead = !__all_sync(kFull, mbar_wait(&sh.empty[s], phase, &sh.abort));
+          dead = !__all_sync(kFull, mbar_wait(&sh.empty[s], phase, &sh.abort, g.wait_limit));
           if (dead) { sh.abort = 1; break; }
         }
         unsigned char *a = ring + (size_t)s * S::stage_bytes;
@@ -523,8 +535,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (++s == R) { s = 0; phase ^= 1; }
       }
     }
-    if (dead || sh.abort) {
-      const volatile int *never = &sh.never;
+    meet_in_cta();
+    if (sh.abort) {
+      const volatile int *never = &sh.never;  // the flag itself must not end this wait
       for (uint32_t j = (issued > (uint32_t)R ? issued - R : 0); j < issued; ++j) mbar_wait(&sh.full[j % R], (j / R) & 1, never);
       if (lane == 0 && g.sticky != nullptr) {
         volatile int32_t *r = g.sticky;
@@ -543,8 +556,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const Place p = place(tile);
       for (int kb = p.k0; kb < p.k1; ++kb, ++blocks) {
         bool ok = true;
-        if (blocks >= (uint32_t)B) ok = mbar_wait(&sh.acc_empty[buf], free_phase, &sh.abort);
-        ok = ok && mbar_wait(&sh.full[s], full_phase, &sh.abort);
+        if (blocks >= (uint32_t)B) ok = mbar_wait(&sh.acc_empty[buf], free_phase, &sh.abort, g.wait_limit);
+        ok = ok && mbar_wait(&sh.full[s], full_phase, &sh.abort, g.wait_limit);
         dead = !__all_sync(kFull, ok);
         if (dead) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -562,11 +575,15 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (++buf == B) { buf = 0; free_phase ^= 1; }
       }
     }
-    if (dead && blocks > 0) {  // the MMAs in flight still read shared memory and write tensor memory
+    meet_in_cta();
+    if (sh.abort && blocks > 0) {  // the MMAs in flight still read shared memory and write tensor memory
       if (elect_one()) mma_commit(&sh.drained);
       __syncwarp();
       mbar_wait(&sh.drained, 0, &sh.never);
     }
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::tmem_columns) : "memory");
+  } else {
+    meet_in_cta();
   }
   } else {
     if constexpr (S::split_registers) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -624,7 +641,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         } else if (tile < g.tiles) {
           aim(p);
         }
-        dead = !__all_sync(kFull, mbar_wait(&sh.acc_full[buf], (it / B) & 1, &sh.abort));
+        dead = !__all_sync(kFull, mbar_wait(&sh.acc_full[buf], (it / B) & 1, &sh.abort, g.wait_limit));
         if (dead) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         float s;  // volatile: stays behind the wait.  Left to the compiler the product moved up to where its
@@ -702,12 +719,18 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       }
     }
     if (g.unit == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    meet_in_cta();
+    if (sh.abort) {
+      for (tile = blockIdx.x; tile < g.tiles; tile += gridDim.x) {
+        p = place(tile);
+        const int64_t row0 = (int64_t)p.mt * kTileM;
+        const int rows = (int)min((int64_t)kTileM, g.M - row0), cols = min(kTileN, g.N - p.nt * kTileN);
+        OutT *out = reinterpret_cast<OutT *>(g.out) + ((int64_t)p.sp * g.out_rows + row0) * g.N + p.nt * kTileN;
+        for (int i = threadIdx.x - 128; i < rows * cols; i += 32 * S::epilogue_warps)
+          out[(int64_t)(i / cols) * g.N + i % cols] = (OutT)__int_as_float(0x7fffffff);
+      }
+    }
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::tmem_columns) : "memory");
 }
 
 // out = sum over the pieces of K (in their order) + bias, rounded once.
@@ -727,6 +750,15 @@ split_sum_kernel(const float *__restrict__ part, int splits, int64_t stride, int
 // launches
 // ---------------------------------------------------------------------------
 struct MatmulPlan { int tile_n, splits; };
+
+// Polls of a barrier before a wait of the product gives up.  OT_B200_WAIT_LIMIT, read at every
+// call, lowers it: with 0 every wait gives up at once, which is how the way out is tested.  The
+// waits for copies and MMAs in flight keep kSpinLimit.
+int wait_limit() {
+  const char *e = getenv("OT_B200_WAIT_LIMIT");
+  const long n = e ? strtol(e, nullptr, 10) : kSpinLimit;
+  return n < 0 ? 0 : (n > kSpinLimit ? kSpinLimit : (int)n);
+}
 
 // Rows of one piece's partial sums: whole row tiles, so that a store never reaches the next piece's.
 int64_t whole_tiles(int64_t M) { return (M + kTileM - 1) / kTileM * kTileM; }
@@ -882,6 +914,7 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
   if (need > 0 && (!d_workspace || workspace_bytes < need || !aligned16(d_workspace)))
     return fail(OT_B200_ERR_WORKSPACE, "ot_b200_fp8_matmul: workspace missing, misaligned or smaller than %llu bytes", (unsigned long long)need);
   MatmulArgs g;
+  g.wait_limit = wait_limit();
   const int begun = begin_reported_call(flags, &g.sticky, &g.seq);
   if (begun) return begun;
   const MatmulPlan p = plan_matmul(M, N, K, sm_count());

@@ -8,15 +8,15 @@
 
 namespace otb {
 
-constexpr int kSpinLimit = 1 << 22;
+constexpr int kSpinLimit = 1 << 22;  // polls of a barrier before a wait gives up
 
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Bounded wait; false when it ran out, or when another role of the CTA has given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, const volatile int *abort) {
-  for (int spin = 0; spin < kSpinLimit; ++spin) {
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, const volatile int *abort, int limit = kSpinLimit) {
+  for (int spin = 0; spin < limit; ++spin) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((spin & 255) == 255 && *abort) return false;
   }
