@@ -496,7 +496,7 @@ namespace otb {
 // fused_linear.cu
 cudaError_t launch_linear_gradient(const Problem &p, const void *x, const void *w, const float *bias,
                                    int D, void *grad, const float *d_scale, float scale_host,
-                                   cudaStream_t s);
+                                   int32_t *sticky, int32_t seq, cudaStream_t s);
 }  // namespace otb
 
 using namespace otb;
@@ -745,14 +745,13 @@ int ot_b200_backward_linear(const void *d_x, const void *d_w, const float *d_bia
   p.logits = nullptr; p.targets = nullptr; p.T = nullptr; p.U = nullptr;
   p.N = N; p.rows = rows; p.V = V; p.max_u = max_u; p.blank = blank; p.flags = flags;
   p.ws = static_cast<char *>(const_cast<void *>(d_workspace));
-  {  // a pending record of a failed call (the forward half of this very loss, perhaps) is raised here
-    int32_t *sticky = nullptr;
-    int32_t seq = 0;
-    rc = begin_reported_call(flags, &sticky, &seq);
-    if (rc) return rc;
-  }
+  // a pending record of a failed call (the forward half of this very loss, perhaps) is raised here
+  int32_t *sticky = nullptr;
+  int32_t seq = 0;
+  rc = begin_reported_call(flags, &sticky, &seq);
+  if (rc) return rc;
   const cudaError_t e = launch_linear_gradient(p, d_x, d_w, d_bias, D, d_grad_logits, d_scale, (float)scale_host,
-                                               static_cast<cudaStream_t>(stream));
+                                               sticky, seq, static_cast<cudaStream_t>(stream));
   if (e == cudaErrorNotSupported)
     return fail(OT_B200_ERR_CUDA, "ot_b200_backward_linear: the driver's tensor-map encoder is not available or refused the operands");
   if (e != cudaSuccess) return fail_cuda(e, "launch linear gradient");

@@ -21,7 +21,6 @@
 #include <cuda_fp8.h>
 #include <stdarg.h>
 #include <stdio.h>
-#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
@@ -750,15 +749,6 @@ split_sum_kernel(const float *__restrict__ part, int splits, int64_t stride, int
 // launches
 // ---------------------------------------------------------------------------
 struct MatmulPlan { int tile_n, splits; };
-
-// Polls of a barrier before a wait of the product gives up.  OT_B200_WAIT_LIMIT, read at every
-// call, lowers it: with 0 every wait gives up at once, which is how the way out is tested.  The
-// waits for copies and MMAs in flight keep kSpinLimit.
-int wait_limit() {
-  const char *e = getenv("OT_B200_WAIT_LIMIT");
-  const long n = e ? strtol(e, nullptr, 10) : kSpinLimit;
-  return n < 0 ? 0 : (n > kSpinLimit ? kSpinLimit : (int)n);
-}
 
 // Rows of one piece's partial sums: whole row tiles, so that a store never reaches the next piece's.
 int64_t whole_tiles(int64_t M) { return (M + kTileM - 1) / kTileM * kTileM; }

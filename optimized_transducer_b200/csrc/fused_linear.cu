@@ -30,10 +30,12 @@
 //               by a select tree) while the MMA warp fills the other accumulator;
 //               the two halves of a row meet in shared memory at the end of its tile
 //
-// Every wait on an mbarrier is bounded; on expiry the CTA raises its abort flag,
-// records status word kStatusCopyTimeout, all roles leave their loops, the
-// producer waits (bounded) for its copies in flight, TMEM is freed and the CTA
-// returns.
+// Every wait on an mbarrier is bounded; on expiry the CTA raises its abort flag and
+// all roles leave their loops and meet.  Behind that barrier, whichever role gave
+// up, the copies and MMAs in flight are waited for (bounded), status word
+// kStatusCopyTimeout is set (the gradient kernel, behind which nobody reads it,
+// fills its tiles with NaN and writes the record that the next call raises), TMEM
+// is freed and the CTA returns.
 #include "ot_common.cuh"
 #include "tensor_core.cuh"
 
@@ -79,8 +81,11 @@ struct FusedShared {
   uint64_t empty[kRing];       // MMA -> TMA: the stage's MMAs have completed
   uint64_t acc_full[2];        // MMA -> epilogue: the accumulator is complete
   uint64_t acc_empty[2];       // epilogue -> MMA: the accumulator has been read (one arrival per epilogue thread)
+  uint64_t drained;            // every MMA issued so far has completed (after an abort)
   uint32_t tmem_base;
-  volatile int abort;
+  volatile int abort;          // a wait ran out: every role leaves its loop
+  int never;
+  uint32_t issued;             // stages that the producer has requested
   float4 half[kTileM];         // (max, sum, blank entry, target entry) of the rows' second halves
 };
 
@@ -98,12 +103,26 @@ __device__ __forceinline__ float pick32(const float (&x)[32], int idx) {
   return (idx & 1) ? d[1] : d[0];
 }
 
+// Barrier 2 over `threads` threads; true for all of them when `mine` is for any.
+__device__ __forceinline__ bool any_of_barrier_2(int threads, int mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, 2, %1, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"(threads), "r"(mine) : "memory");
+  return any != 0;
+}
+
 // What the gradient variant needs besides the operands (see linear_gradient_kernel).
 struct GradArgs {
   const CoefA<float> *coef;   // per-row coefficient records of the forward half
   __nv_bfloat16 *grad;        // (rows, V) out
   const float *d_scale;       // device scalar or NULL
   float scale_host;
+  int32_t *sticky;            // error record, or NULL
+  int32_t seq;
 };
 
 // Body of both kernels.  kGrad == false: stage 1 (den, lp).  kGrad == true: the
@@ -115,7 +134,7 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
             const int32_t *__restrict__ Tl, const int32_t *__restrict__ Ul,
             const int64_t *__restrict__ split, const int64_t *__restrict__ cell_split,
             int32_t *__restrict__ status, int N, int64_t rows, int D, int V, int max_u,
-            int blank, float *__restrict__ den, float *__restrict__ lp, const GradArgs ga) {
+            int blank, float *__restrict__ den, float *__restrict__ lp, int limit, const GradArgs ga) {
   constexpr int R = kGrad ? kRingGrad : kRing;  // stages of the operand ring
   constexpr int kEW = kGrad ? kGradEpilogueWarps : kEpilogueWarps;  // epilogue warps
   constexpr int kThreadsHere = 64 + 32 * kEW;
@@ -138,7 +157,10 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
   if (threadIdx.x == 0) {
     for (int i = 0; i < R; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], 32 * kEW); }
+    mbar_init(&sh.drained, 1);
     sh.abort = 0;
+    sh.never = 0;
+    sh.issued = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -165,7 +187,7 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
       for (int ct = 0; ct < col_tiles && !sh.abort; ++ct) {
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % R;
-          if (it >= R && !mbar_wait(&sh.empty[s], ((it / R) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+          if (it >= R && !mbar_wait(&sh.empty[s], ((it / R) - 1) & 1, &sh.abort, limit)) { sh.abort = 1; break; }
           unsigned char *a = ring + (size_t)s * kStageBytes;
           mbar_expect_tx(&sh.full[s], kStageBytes);
           // rows / columns past the ends of x and w are filled with zeros by the copy
@@ -174,25 +196,19 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
         }
       }
     }
-    if (sh.abort) {  // let the copies in flight land before the CTA gives its shared memory back
-      __shared__ int never;  // the drain must not stop because of the abort flag itself
-      never = 0;
-      const volatile int *nullptr_abort = &never;
-      for (uint32_t j = (it > R ? it - R : 0); j < it; ++j) mbar_wait(&sh.full[j % R], (j / R) & 1, nullptr_abort);
-      atomicCAS(status + kStatusCopyTimeout, 0, 1);
-    }
+    sh.issued = it;
   } else if (run && warp == 1 && lane == 0) {
     // ------------------------------- MMA issuer -------------------------------
     uint32_t it = 0, acc_it = 0;  // stages consumed, accumulators filled
     for (int64_t tile = blockIdx.x; tile < row_tiles && !sh.abort; tile += gridDim.x) {
       for (int ct = 0; ct < col_tiles && !sh.abort; ++ct, ++acc_it) {
         const int buf = acc_it & 1;
-        if (acc_it >= 2 && !mbar_wait(&sh.acc_empty[buf], ((acc_it >> 1) - 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+        if (acc_it >= 2 && !mbar_wait(&sh.acc_empty[buf], ((acc_it >> 1) - 1) & 1, &sh.abort, limit)) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + (uint32_t)(buf * kTileN);
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % R;
-          if (!mbar_wait(&sh.full[s], (it / R) & 1, &sh.abort)) { sh.abort = 1; break; }
+          if (!mbar_wait(&sh.full[s], (it / R) & 1, &sh.abort, limit)) { sh.abort = 1; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t a = smem_u32(ring + (size_t)s * kStageBytes);
           const uint64_t da = smem_desc(a), db = smem_desc(a + kBytesA);
@@ -205,7 +221,6 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
         mma_commit(&sh.acc_full[buf]);
       }
     }
-    if (sh.abort) atomicCAS(status + kStatusCopyTimeout, 0, 1);
   } else if (run && warp >= 2) {
    if constexpr (kGrad) {
     // --------------------------- epilogue, gradient ---------------------------
@@ -223,7 +238,8 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
     const float mul = fold ? 1.f : scale_all;
     const float k_scale = fold ? __log2f(scale_all) : 0.f;
     uint32_t acc_it = 0;
-    for (int64_t tile = blockIdx.x; tile < row_tiles && !sh.abort; tile += gridDim.x) {
+    bool dead = false;  // the same for all lanes: the reads of tensor memory are warp-wide
+    for (int64_t tile = blockIdx.x; tile < row_tiles && !dead; tile += gridDim.x) {
       const int64_t row = tile * kTileM + r_in_tile;
       const bool live = row < rows;
       bool zero_row = true;
@@ -240,9 +256,10 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
         tgt = ids.x >= 0 ? ids.x : -1;
       }
       uint32_t *mine = out_s + (warp - 2) * 32 * kOutPitch;
-      for (int ct = 0; ct < col_tiles && !sh.abort; ++ct, ++acc_it) {
+      for (int ct = 0; ct < col_tiles; ++ct, ++acc_it) {
         const int buf = acc_it & 1;
-        if (!mbar_wait(&sh.acc_full[buf], (acc_it >> 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+        dead = !__all_sync(kFull, mbar_wait(&sh.acc_full[buf], (acc_it >> 1) & 1, &sh.abort, limit));
+        if (dead) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kTileN);
         // The warp's chunks of this accumulator (c = part, part + kParts, ...); the
@@ -322,7 +339,6 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
         }
       }
     }
-    if (sh.abort && lane == 0) atomicCAS(status + kStatusCopyTimeout, 0, 1);
    } else {
     // -------------------------------- epilogue --------------------------------
     // TMEM lanes 32*(warp % 4) .. +31 are the ones a warp may read; the two warps of
@@ -332,7 +348,8 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
     const int r_in_tile = quarter * 32 + lane;
     const float ninf = neg_inf<float>();
     uint32_t acc_it = 0;
-    for (int64_t tile = blockIdx.x; tile < row_tiles && !sh.abort; tile += gridDim.x) {
+    bool dead = false;  // the same for all lanes, as above
+    for (int64_t tile = blockIdx.x; tile < row_tiles; tile += gridDim.x) {
       const int64_t row = tile * kTileM + r_in_tile;
       const bool live = row < rows;
       int tsym = -1;
@@ -346,9 +363,10 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
         cell = __ldg(cell_split + b) + cell_pos<false>(t, u, U1);
       }
       float m = ninf, ssum = 0.f, g_blank = ninf, g_sym = ninf;
-      for (int ct = 0; ct < col_tiles && !sh.abort; ++ct, ++acc_it) {
+      for (int ct = 0; ct < col_tiles; ++ct, ++acc_it) {
         const int buf = acc_it & 1;
-        if (!mbar_wait(&sh.acc_full[buf], (acc_it >> 1) & 1, &sh.abort)) { sh.abort = 1; break; }
+        dead = !__all_sync(kFull, mbar_wait(&sh.acc_full[buf], (acc_it >> 1) & 1, &sh.abort, limit));
+        if (dead) { sh.abort = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kTileN);
 #pragma unroll 1
@@ -398,9 +416,11 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
         mbar_arrive(&sh.acc_empty[buf]);  // one arrival per epilogue thread: the accumulator has been read
       }
       // The two halves of a row meet: part 1 leaves its (max, sum, entries), part 0 merges and writes.
+      // Where they meet they also agree on leaving: with the flag read by each warp for itself
+      // one could leave while another goes on to the next of these barriers.
       if (part == 1) sh.half[r_in_tile] = make_float4(m, ssum, g_blank, g_sym);
-      asm volatile("bar.sync 2, %0;" ::"r"(32 * kEpilogueWarps) : "memory");
-      if (part == 0 && live && !sh.abort) {
+      if (any_of_barrier_2(32 * kEpilogueWarps, dead)) break;
+      if (part == 0 && live) {
         const float4 o = sh.half[r_in_tile];
         const float mm = fmaxf(m, o.x);
         float tot = 0.f;
@@ -413,13 +433,39 @@ linear_body(const CUtensorMap &map_x, const CUtensorMap &map_w,
       }
       asm volatile("bar.sync 2, %0;" ::"r"(32 * kEpilogueWarps) : "memory");  // half[] may be overwritten again
     }
-    if (sh.abort && lane == 0) atomicCAS(status + kStatusCopyTimeout, 0, 1);
    }
   }
   // Everybody meets here, whatever happened; then tensor memory goes back.
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (sh.abort) {
+    if (threadIdx.x == 0) {  // the copies in flight land before the CTA gives its shared memory back
+      for (uint32_t j = (sh.issued > R ? sh.issued - R : 0); j < sh.issued; ++j)
+        mbar_wait(&sh.full[j % R], (j / R) & 1, &sh.never);  // (the flag itself must not end this wait)
+      atomicCAS(status + kStatusCopyTimeout, 0, 1);
+      if (kGrad && ga.sticky != nullptr) {  // no later kernel of this call reads the status
+        volatile int32_t *r = ga.sticky;
+        r[1] = 0;
+        r[2] = ga.seq;
+        __threadfence_system();
+        r[0] = OT_B200_COPY_TIMEOUT;
+      }
+    }
+    if (warp == 1 && lane == 0) {  // (the thread that issued them) the MMAs in flight read it too, and write tensor memory
+      mma_commit(&sh.drained);
+      mbar_wait(&sh.drained, 0, &sh.never);
+    }
+    __syncwarp();
+    if (kGrad) {  // the gradient of the CTA's tiles is NaN
+      for (int64_t tile = blockIdx.x; tile < row_tiles; tile += gridDim.x) {
+        const int64_t words = min((int64_t)kTileM, rows - tile * kTileM) * V / 2;
+        uint32_t *g = reinterpret_cast<uint32_t *>(ga.grad + tile * kTileM * V);
+        for (int64_t i = threadIdx.x; i < words; i += kThreadsHere) g[i] = 0x7fff7fffu;
+      }
+    }
+    __syncwarp();
+  }
   if (run && threadIdx.x == 0) trace_end(status, kGrad ? kStageGradient : kStageLogprob);
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
@@ -439,9 +485,9 @@ linear_logprob_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                       const int32_t *__restrict__ Tl, const int32_t *__restrict__ Ul,
                       const int64_t *__restrict__ split, const int64_t *__restrict__ cell_split,
                       int32_t *__restrict__ status, int N, int64_t rows, int D, int V, int max_u,
-                      int blank, float *__restrict__ den, float *__restrict__ lp) {
+                      int blank, float *__restrict__ den, float *__restrict__ lp, int limit) {
   linear_body<false>(map_x, map_w, bias, targets, Tl, Ul, split, cell_split, status, N, rows, D, V, max_u,
-                     blank, den, lp, GradArgs{nullptr, nullptr, nullptr, 1.f});
+                     blank, den, lp, limit, GradArgs{nullptr, nullptr, nullptr, 1.f, nullptr, 0});
 }
 
 // The gradient of -sum(scores) with respect to the logits, times `scale`, in
@@ -456,9 +502,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 linear_gradient_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                        const float *__restrict__ bias, int32_t *__restrict__ status, int64_t rows, int D,
                        int V, int blank, const CoefA<float> *__restrict__ coef,
-                       __nv_bfloat16 *__restrict__ grad, const float *__restrict__ d_scale, float scale_host) {
+                       __nv_bfloat16 *__restrict__ grad, const float *__restrict__ d_scale, float scale_host,
+                       int limit, int32_t *sticky, int32_t seq) {
   linear_body<true>(map_x, map_w, bias, nullptr, nullptr, nullptr, nullptr, nullptr, status, 0, rows, D, V, 0,
-                    blank, nullptr, nullptr, GradArgs{coef, grad, d_scale, scale_host});
+                    blank, nullptr, nullptr, limit, GradArgs{coef, grad, d_scale, scale_host, sticky, seq});
 }
 
 // (outer, inner) bfloat16 matrix, row-major; boxes of box_outer x 64 elements.
@@ -491,7 +538,8 @@ cudaError_t launch_linear_logprob(const Problem &p, const void *x, const void *w
                  p.targets, p.T, p.U, reinterpret_cast<const int64_t *>(p.ws + p.lay.split),
                  reinterpret_cast<const int64_t *>(p.ws + p.lay.cell_split),
                  reinterpret_cast<int32_t *>(p.ws + p.lay.status), p.N, p.rows, D, p.V, p.max_u, p.blank,
-                 reinterpret_cast<float *>(p.ws + p.lay.den), reinterpret_cast<float *>(p.ws + p.lay.lp));
+                 reinterpret_cast<float *>(p.ws + p.lay.den), reinterpret_cast<float *>(p.ws + p.lay.lp),
+                 wait_limit());
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -499,7 +547,7 @@ cudaError_t launch_linear_logprob(const Problem &p, const void *x, const void *w
 // linear_gradient_kernel).  V must be a multiple of 4 and grad 8-byte aligned.
 cudaError_t launch_linear_gradient(const Problem &p, const void *x, const void *w, const float *bias,
                                    int D, void *grad, const float *d_scale, float scale_host,
-                                   cudaStream_t s) {
+                                   int32_t *sticky, int32_t seq, cudaStream_t s) {
   CUtensorMap map_x, map_w;
   if (!make_map(&map_x, x, (uint64_t)p.rows, (uint64_t)D, kTileM) ||
       !make_map(&map_w, w, (uint64_t)p.V, (uint64_t)D, kTileN))
@@ -516,7 +564,7 @@ cudaError_t launch_linear_gradient(const Problem &p, const void *x, const void *
   e = launch_pdl(linear_gradient_kernel, grid, (unsigned)kGradThreads, smem, s, map_x, map_w, bias,
                  reinterpret_cast<int32_t *>(p.ws + p.lay.status), p.rows, D, p.V, p.blank,
                  reinterpret_cast<const CoefA<float> *>(p.ws + p.lay.coef),
-                 static_cast<__nv_bfloat16 *>(grad), d_scale, scale_host);
+                 static_cast<__nv_bfloat16 *>(grad), d_scale, scale_host, wait_limit(), sticky, seq);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -3,12 +3,22 @@
 #pragma once
 
 #include <cuda.h>  // CUtensorMap and its enums only; the encoder is looked up at run time
+#include <stdlib.h>
 
 #include "ot_common.cuh"
 
 namespace otb {
 
 constexpr int kSpinLimit = 1 << 22;  // polls of a barrier before a wait gives up
+
+// The same for the waits of the roles on each other: OT_B200_WAIT_LIMIT, read at every call,
+// lowers it (with 0 every wait gives up at once, which is how the way out is tested).  The waits
+// for copies and MMAs in flight keep kSpinLimit.
+inline int wait_limit() {
+  const char *e = getenv("OT_B200_WAIT_LIMIT");
+  const long n = e ? strtol(e, nullptr, 10) : kSpinLimit;
+  return n < 0 ? 0 : (n > kSpinLimit ? kSpinLimit : (int)n);
+}
 
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
