@@ -885,9 +885,17 @@ int ot_b200_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, uint64_t
   return OT_B200_OK;
 }
 
-int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a, const void *d_b, int64_t b_pitch,
-                       const float *d_scale_b, const float *d_bias, int64_t M, int64_t N, int64_t K, uint32_t flags,
-                       void *d_workspace, uint64_t workspace_bytes, void *d_out, void *stream) {
+// Which error record a call writes to, or none: what begin_reported_call found.  An entry point
+// of several launches asks before the first of them.
+struct Report {
+  int32_t *sticky = nullptr;
+  int32_t seq = 0;
+};
+
+// The product; `report` NULL: it asks for the error record itself.
+static int matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a, const void *d_b, int64_t b_pitch,
+                  const float *d_scale_b, const float *d_bias, int64_t M, int64_t N, int64_t K, uint32_t flags,
+                  void *d_workspace, uint64_t workspace_bytes, void *d_out, const Report *report, void *stream) {
   const uint32_t types = flags & (OT_B200_BF16 | OT_B200_FP16);
   if ((flags & ~(OT_B200_BF16 | OT_B200_FP16 | OT_B200_REPORT_ERRORS)) || (types & (types - 1)))
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_fp8_matmul: flags may hold one of OT_B200_BF16 and OT_B200_FP16, and OT_B200_REPORT_ERRORS");
@@ -905,8 +913,13 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
     return fail(OT_B200_ERR_WORKSPACE, "ot_b200_fp8_matmul: workspace missing, misaligned or smaller than %llu bytes", (unsigned long long)need);
   MatmulArgs g;
   g.wait_limit = wait_limit();
-  const int begun = begin_reported_call(flags, &g.sticky, &g.seq);
-  if (begun) return begun;
+  if (report != nullptr) {
+    g.sticky = report->sticky;
+    g.seq = report->seq;
+  } else {
+    const int begun = begin_reported_call(flags, &g.sticky, &g.seq);
+    if (begun) return begun;
+  }
   const MatmulPlan p = plan_matmul(M, N, K, sm_count());
   CUtensorMap ma, mb;
   if (!make_tensor_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, d_a, (uint64_t)M, (uint64_t)K, (uint64_t)a_pitch, kTileM, kScaleBlock) ||
@@ -951,6 +964,13 @@ int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a,
   return OT_B200_OK;
 }
 
+int ot_b200_fp8_matmul(const void *d_a, int64_t a_pitch, const float *d_scale_a, const void *d_b, int64_t b_pitch,
+                       const float *d_scale_b, const float *d_bias, int64_t M, int64_t N, int64_t K, uint32_t flags,
+                       void *d_workspace, uint64_t workspace_bytes, void *d_out, void *stream) {
+  return matmul(d_a, a_pitch, d_scale_a, d_b, b_pitch, d_scale_b, d_bias, M, N, K, flags, d_workspace, workspace_bytes, d_out,
+                nullptr, stream);
+}
+
 // Bytes from row to row of a quantised matrix: whole cache lines, so that the 128 bytes of a
 // row that one TMA box takes lie in one line and not in two.
 static int64_t row_pitch(int64_t n) { return (n + 127) / 128 * 128; }
@@ -979,14 +999,17 @@ int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_
   if (rc) return rc;
   if (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0)
     return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_logits: workspace missing, not 256-byte aligned or smaller than %llu bytes", (unsigned long long)need);
+  Report report;
+  rc = begin_reported_call(out_flags, &report.sticky, &report.seq);
+  if (rc) return rc;
   joiner_layout(rows, D, &scale_off, &product_off);
   char *ws = static_cast<char *>(d_workspace);
   const int64_t pitch = row_pitch(D);
   float *scale = reinterpret_cast<float *>(ws + scale_off);
   rc = ot_b200_fp8_quantize(d_x, rows, D, row_stride, x_flags, OT_B200_FP8_ROWS, ws, pitch, scale, nullptr, 0, nullptr, nullptr, nullptr, stream);
   if (rc) return rc;
-  return ot_b200_fp8_matmul(ws, pitch, scale, d_w, w_pitch, d_w_scale, d_bias, rows, V, D, out_flags,
-                            ws + product_off, workspace_bytes - product_off, d_out, stream);
+  return matmul(ws, pitch, scale, d_w, w_pitch, d_w_scale, d_bias, rows, V, D, out_flags, ws + product_off,
+                workspace_bytes - product_off, d_out, &report, stream);
 }
 
 // The training form's buffers, one behind the other (0 bytes where a gradient is not asked for).
@@ -1052,6 +1075,9 @@ int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64
   if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0 ||
       (t.saved && (!d_saved || reinterpret_cast<uintptr_t>(d_saved) % 256 != 0)))
     return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_train_forward: a buffer is missing or not 256-byte aligned");
+  Report report;
+  rc = begin_reported_call(out_flags, &report.sticky, &report.seq);
+  if (rc) return rc;
   char *ws = static_cast<char *>(d_workspace), *saved = static_cast<char *>(d_saved);
   const auto at = [](char *base, uint64_t off) { return reinterpret_cast<float *>(base + off); };
   rc = ot_b200_fp8_quantize(d_w, V, D, w_stride, w_flags, need_x ? OT_B200_FP8_SQUARES_BOTH : OT_B200_FP8_SQUARES,
@@ -1062,8 +1088,8 @@ int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64
                               ws + t.x, row_pitch(D), at(ws, t.x_scale), need_w ? saved + t.xt : nullptr,
                               need_w ? row_pitch(rows) : 0, need_w ? at(saved, t.xt_scale) : nullptr, nullptr, nullptr, stream);
   if (!rc)
-    rc = ot_b200_fp8_matmul(ws + t.x, row_pitch(D), at(ws, t.x_scale), ws + t.w, row_pitch(D), at(ws, t.w_scale), d_bias, rows, V, D,
-                            out_flags, ws + t.f_product, t.forward - t.f_product, d_out, stream);
+    rc = matmul(ws + t.x, row_pitch(D), at(ws, t.x_scale), ws + t.w, row_pitch(D), at(ws, t.w_scale), d_bias, rows, V, D, out_flags,
+                ws + t.f_product, t.forward - t.f_product, d_out, &report, stream);
   return rc;
 }
 
@@ -1078,6 +1104,9 @@ int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int6
     return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_train_backward: a buffer is missing or not 256-byte aligned");
   if (flags & ~OT_B200_REPORT_ERRORS)
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_joiner_train_backward: flags may hold OT_B200_REPORT_ERRORS");
+  Report report;
+  rc = begin_reported_call(flags, &report.sticky, &report.seq);
+  if (rc) return rc;
   char *ws = static_cast<char *>(d_workspace), *saved = static_cast<char *>(const_cast<void *>(d_saved));
   const auto at = [](char *base, uint64_t off) { return reinterpret_cast<float *>(base + off); };
   const bool columns = d_gw || d_gb;
@@ -1085,11 +1114,11 @@ int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int6
                             row_pitch(V), at(ws, t.g_scale), columns ? ws + t.gt : nullptr, columns ? row_pitch(rows) : 0,
                             columns ? at(ws, t.gt_scale) : nullptr, d_gb ? at(ws, t.sums) : nullptr, d_gb, stream);
   if (!rc && d_gx)
-    rc = ot_b200_fp8_matmul(ws + t.g, row_pitch(V), at(ws, t.g_scale), saved + t.wt, row_pitch(V), at(saved, t.wt_scale), nullptr, rows,
-                            D, V, x_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gx, stream);
+    rc = matmul(ws + t.g, row_pitch(V), at(ws, t.g_scale), saved + t.wt, row_pitch(V), at(saved, t.wt_scale), nullptr, rows, D, V,
+                x_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gx, &report, stream);
   if (!rc && d_gw)
-    rc = ot_b200_fp8_matmul(ws + t.gt, row_pitch(rows), at(ws, t.gt_scale), saved + t.xt, row_pitch(rows), at(saved, t.xt_scale), nullptr,
-                            V, D, rows, w_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gw, stream);
+    rc = matmul(ws + t.gt, row_pitch(rows), at(ws, t.gt_scale), saved + t.xt, row_pitch(rows), at(saved, t.xt_scale), nullptr, V, D, rows,
+                w_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gw, &report, stream);
   return rc;
 }
 

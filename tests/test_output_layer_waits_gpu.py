@@ -77,3 +77,42 @@ def test_waits_that_give_up_halfway(limit, monkeypatch):
         else:
             ot.check_inputs(DEV)
         assert torch.equal(ot.joiner_logits(x, w, b), want)
+
+
+def test_a_pending_record_is_raised_before_anything_is_launched(monkeypatch):
+    """The record of a failed call reaches the next call at its entry: none of that call's buffers is written."""
+    import ctypes
+
+    from optimized_transducer_b200 import _lib
+
+    lib, rows, d, v = _lib.load(), 50, 96, 40
+    x, w, b = _operands(rows, d, v)
+    wt = torch.randn(v, d, device=DEV)
+    g = torch.randn(rows, v, device=DEV)
+    n = [ctypes.c_uint64() for _ in range(4)]
+    _lib.check(lib.ot_b200_joiner_train_bytes(rows, d, v, 1, 1, 1, *[ctypes.byref(i) for i in n[:3]]))
+    _lib.check(lib.ot_b200_joiner_logits_workspace_bytes(rows, d, v, ctypes.byref(n[3])))
+    saved, fwd, bwd, ws = (torch.full((i.value,), 0xAB, dtype=torch.uint8, device=DEV) for i in n)
+    out, gx, gw, gb = (torch.full(s, 7.0, device=DEV) for s in ((rows, v), (rows, d), (v, d), (v,)))
+    buffers = (saved, fwd, bwd, ws, out, gx, gw, gb)
+    stream, on = torch.cuda.current_stream().cuda_stream, _lib.REPORT_ERRORS
+    calls = [
+        lambda: lib.ot_b200_joiner_logits(x.data_ptr(), rows, d, d, _lib.BF16, w.data.data_ptr(), w.data.stride(0), w.scale.data_ptr(), v,
+                                          b.data_ptr(), on, ws.data_ptr(), ws.numel(), out.data_ptr(), stream),
+        lambda: lib.ot_b200_joiner_train_forward(x.data_ptr(), rows, d, d, _lib.BF16, wt.data_ptr(), v, d, 0, b.data_ptr(), on, 1, 1,
+                                                 saved.data_ptr(), fwd.data_ptr(), out.data_ptr(), stream),
+        lambda: lib.ot_b200_joiner_train_backward(g.data_ptr(), rows, v, v, 0, d, saved.data_ptr(), gx.data_ptr(), 0, gw.data_ptr(), 0,
+                                                  gb.data_ptr(), on, bwd.data_ptr(), stream),
+    ]
+    for call in calls:
+        monkeypatch.setenv("OT_B200_WAIT_LIMIT", "0")
+        ot.joiner_logits(x, w, b)
+        torch.cuda.synchronize()
+        monkeypatch.delenv("OT_B200_WAIT_LIMIT")
+        before = [t.clone() for t in buffers]
+        assert call() == _lib.ERR_INPUT and "did not complete in time" in _lib.last_error()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(before, buffers))
+        assert call() == _lib.OK                      # raised once; this call runs
+        torch.cuda.synchronize()
+    assert float((gb - g.sum(0)).abs().max()) <= 1e-4
