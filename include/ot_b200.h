@@ -376,7 +376,8 @@ int ot_b200_sample(const void *d_logits, int64_t rows, int32_t V, int64_t row_st
  * place nothing is written when the factor is 1.  Tensors must not overlap (one listed
  * twice is refused), nor an output another tensor.  apply = 0: only the norm.
  * *d_norm (float) receives the norm; sums are taken in double over groups of at most 32
- * elements, in a fixed order.  A norm that is not finite scales as it does in torch
+ * elements, in a fixed order.  The factor comes from the norm in double; it is rounded to
+ * float for gradients of up to 32 bits and stays a double for double ones.  A norm that is not finite scales as it does in torch
  * (infinite: by 0; NaN: by NaN).  The workspace (8-byte aligned) may be reused by the next
  * call on the same stream.  Callable in a stream capture; nothing is copied to the device. */
 typedef enum ot_b200_norm_kind { OT_B200_NORM_INF = 0, OT_B200_NORM_1 = 1, OT_B200_NORM_2 = 2 } ot_b200_norm_kind;

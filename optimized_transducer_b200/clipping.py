@@ -74,8 +74,9 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
     the factor is 1), or, with ``out`` (one tensor per gradient, same shape and strides,
     any of the types), written there and left as they are.  No two tensors may overlap.
     Tensors that require a gradient are refused: unlike torch's function this one is not
-    given the parameters.  The host does not wait for the device.  As in torch an infinite norm scales by 0 and
-    a NaN one by NaN."""
+    given the parameters.  The factor is taken from the norm in float64 (float64 gradients are
+    scaled in float64, the others in float32); what is returned is the norm in float32.  The host
+    does not wait for the device.  As in torch an infinite norm scales by 0 and a NaN one by NaN."""
     who = "clip_grad_norm_"
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"{who}: max_norm must not be negative or a NaN, got {max_norm}")

@@ -281,7 +281,7 @@ apply_kernel(const __grid_constant__ ClipTable<kMax> tab, const double *__restri
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   // a NaN norm makes the factor a NaN, an infinite one makes it 0
   const double ratio = max_norm / (norm + 1e-6);
-  const double factor = ratio >= 1.0 ? 1.0 : (double)(float)ratio;
+  const double factor = ratio >= 1.0 ? 1.0 : ratio;  // rounded to float where the elements are
   if (in_place && factor == 1.0) return;
   for (uint32_t i = blockIdx.x; i < tab.chunks; i += gridDim.x) {
     const uint32_t c = tab.chunks - 1 - i;  // what the norm pass read last is still in L2
