@@ -217,6 +217,8 @@ template <typename O, typename W> __device__ __forceinline__ O narrow(W x) { ret
 template <> __device__ __forceinline__ double narrow<double, double>(double x) { return x; }
 template <> __device__ __forceinline__ double narrow<double, float>(float x) { return (double)x; }
 template <> __device__ __forceinline__ float narrow<float, double>(double x) { return (float)x; }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16, double>(double x) { return __double2bfloat16(x); }
+template <> __device__ __forceinline__ __half narrow<__half, double>(double x) { return __double2half(x); }
 
 // out = g * factor in the wider of float and the element's type, rounded once.  Vectors of
 // kPer elements: 16 bytes of the wider of the two types, when both sides are aligned for

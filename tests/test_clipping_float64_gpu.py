@@ -56,3 +56,21 @@ def test_float64_beside_other_types():
         assert bool(((got.cpu() - t * factor).abs() <= tol * t.abs() * factor).all())
         ratio = got.cpu() / t                        # one factor for all, to the rounding of the product and the quotient
         assert float(ratio.max() / ratio.min()) - 1 <= 4 * 2.0 ** -53
+
+
+@pytest.mark.parametrize("out_type", [torch.bfloat16, torch.float16, torch.float32])
+def test_float64_gradients_are_rounded_once_into_smaller_types(out_type):
+    """A hair above or below the middle of two neighbours: rounded by way of float32 the hair
+    is lost and the tie goes to the even one."""
+    step = torch.finfo(out_type).eps                  # from 1 to its neighbour
+    hair = 2.0 ** -40
+    above, below = 1 + step / 2 + hair, 1 + 1.5 * step - hair
+    want = {above: 1 + step, below: 1 + step, -above: -1 - step, -below: -1 - step, 1 + step / 2: 1.0, 1 + 1.5 * step: 1 + 2 * step}
+    g = torch.tensor(list(want) * 40, dtype=F64)
+    out = torch.empty(g.numel(), dtype=out_type, device=DEV)
+    ot.clip_grad_norm_([g.to(DEV)], 1e9, out=[out])   # the factor is 1
+    assert torch.equal(out.cpu().double(), torch.tensor(list(want.values()) * 40, dtype=F64))
+    # odd pieces: the elements that vectors leave over
+    for n in (1, 3, 7):
+        ot.clip_grad_norm_([g[:n].to(DEV)], 1e9, out=[out[1:1 + n]])
+        assert torch.equal(out[1:1 + n].cpu().double(), torch.tensor(list(want.values()) * 40, dtype=F64)[:n])
