@@ -15,10 +15,11 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <exception>
+#include <stdexcept>
 #include <vector>
 
 #include "../../include/ot_b200.h"
@@ -40,6 +41,14 @@ template <typename T> PyObject *as_bytes(const std::vector<T> &v) {
   return PyBytes_FromStringAndSize(reinterpret_cast<const char *>(v.data()), (Py_ssize_t)(v.size() * sizeof(T)));
 }
 
+// Runs f; what it throws becomes the Python exception that torch makes of it (a failed
+// allocation torch.OutOfMemoryError).
+template <typename F> PyObject *guarded(F f) {
+  HANDLE_TH_ERRORS
+  return f();
+  END_HANDLE_TH_ERRORS
+}
+
 // describe(list) -> (pointers, counts, type flags, device, index, why): three bytes objects
 // with one 64-, 64- and 32-bit entry per tensor, and the CUDA device all are on; or, at the
 // first tensor that will not do, None four times, its index and "tensor" / "layout" /
@@ -47,8 +56,7 @@ template <typename T> PyObject *as_bytes(const std::vector<T> &v) {
 PyObject *describe(PyObject *, PyObject *list) {
   PyObject *seq = PySequence_Fast(list, "expected a sequence of tensors");
   if (seq == nullptr) return nullptr;
-  PyObject *result = nullptr;
-  try {
+  PyObject *result = guarded([&]() -> PyObject * {
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
     PyObject **items = PySequence_Fast_ITEMS(seq);
     std::vector<int64_t> pointers((size_t)n), counts((size_t)n);
@@ -70,13 +78,9 @@ PyObject *describe(PyObject *, PyObject *list) {
       counts[(size_t)i] = t.numel();
       types[(size_t)i] = flag;
     }
-    if (why != nullptr)
-      result = Py_BuildValue("(OOOOns)", Py_None, Py_None, Py_None, Py_None, i, why);
-    else
-      result = Py_BuildValue("(NNNins)", as_bytes(pointers), as_bytes(counts), as_bytes(types), device, n, "");
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  }
+    if (why != nullptr) return Py_BuildValue("(OOOOns)", Py_None, Py_None, Py_None, Py_None, i, why);
+    return Py_BuildValue("(NNNins)", as_bytes(pointers), as_bytes(counts), as_bytes(types), device, n, "");
+  });
   Py_DECREF(seq);
   return result;
 }
@@ -86,7 +90,7 @@ PyObject *describe(PyObject *, PyObject *list) {
 PyObject *alike(PyObject *, PyObject *args) {
   PyObject *a = nullptr, *b = nullptr;
   if (!PyArg_ParseTuple(args, "O!O!", &PyList_Type, &a, &PyList_Type, &b)) return nullptr;
-  try {
+  return guarded([&]() -> PyObject * {
     const Py_ssize_t n = PyList_GET_SIZE(a) < PyList_GET_SIZE(b) ? PyList_GET_SIZE(a) : PyList_GET_SIZE(b);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject *x = PyList_GET_ITEM(a, i), *y = PyList_GET_ITEM(b, i);
@@ -97,10 +101,7 @@ PyObject *alike(PyObject *, PyObject *args) {
         return PyLong_FromSsize_t(i);
     }
     return PyLong_FromLong(-1);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  });
 }
 
 // writable(list): the index of the first tensor that autograd follows (a parameter, or a
@@ -120,17 +121,15 @@ PyObject *writable(PyObject *, PyObject *list) {
 PyObject *written(PyObject *, PyObject *list) {
   PyObject *seq = PySequence_Fast(list, "expected a sequence of tensors");
   if (seq == nullptr) return nullptr;
-  try {
+  PyObject *result = guarded([&]() -> PyObject * {
     for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) {
       const at::Tensor &t = THPVariable_Unpack(PySequence_Fast_GET_ITEM(seq, i));
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     }
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  }
+    Py_RETURN_NONE;
+  });
   Py_DECREF(seq);
-  if (PyErr_Occurred()) return nullptr;
-  Py_RETURN_NONE;
+  return result;
 }
 
 // ---------------------------------------------------------------------------
@@ -184,15 +183,6 @@ bool plain_vector(const at::Tensor &t, at::ScalarType type, int64_t n, int devic
 }
 
 at::Tensor bytes_on(const at::Tensor &like, uint64_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
-
-template <typename F> PyObject *guarded(F f) {
-  try {
-    return f();
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
-}
 
 // sample(logits, uniforms, temperature, top_k, top_p, min_p): (tokens, logprobs) or None.
 PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
