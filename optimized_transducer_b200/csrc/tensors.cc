@@ -182,7 +182,26 @@ bool plain_vector(const at::Tensor &t, at::ScalarType type, int64_t n, int devic
   return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
 }
 
+// What Fp8Weight checks.  Its tensors may have been resized or exchanged since (Tensor.resize_,
+// Tensor.data), so every call looks again.
+bool plain_weight(const at::Tensor &w, const at::Tensor &scale) {
+  if (w.layout() != at::kStrided || !w.is_cuda() || w.scalar_type() != at::kFloat8_e4m3fn || w.dim() != 2 || w.numel() == 0) return false;
+  const int64_t v = w.size(0), d = w.size(1);
+  return (d == 1 || w.stride(1) == 1) && (v == 1 || (w.stride(0) % 16 == 0 && w.stride(0) >= d)) &&
+         reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && scale.layout() == at::kStrided && scale.is_cuda() &&
+         scale.get_device() == w.get_device() && scale.scalar_type() == at::kFloat && scale.dim() == 2 &&
+         scale.size(0) == (v + 127) / 128 && scale.size(1) == (d + 127) / 128 && scale.is_contiguous();
+}
+
 at::Tensor bytes_on(const at::Tensor &like, uint64_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
+
+// weight(data, scale): whether they are a quantised weight that the kernels can read.
+PyObject *weight(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    return PyBool_FromLong(n == 2 && THPVariable_Check(args[0]) && THPVariable_Check(args[1]) &&
+                           plain_weight(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1])));
+  });
+}
 
 // sample(logits, uniforms, temperature, top_k, top_p, min_p): (tokens, logprobs) or None.
 PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -293,10 +312,11 @@ PyObject *train(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // logits of a quantised weight, or None.
 PyObject *logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
-    if (n != 6 || !THPVariable_Check(args[0]) || !THPDtype_Check(args[4])) Py_RETURN_NONE;
+    if (n != 6 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) || !THPDtype_Check(args[4]))
+      Py_RETURN_NONE;
     const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &scale = THPVariable_Unpack(args[2]);
     const at::ScalarType type = reinterpret_cast<THPDtype *>(args[4])->scalar_type;
-    if (!plain_matrix(x) || float_flag(type) < 0 || w.get_device() != x.get_device() || w.size(1) != x.size(1)) Py_RETURN_NONE;
+    if (!plain_matrix(x) || float_flag(type) < 0 || !plain_weight(w, scale) || w.get_device() != x.get_device() || w.size(1) != x.size(1)) Py_RETURN_NONE;
     const int64_t rows = x.size(0), d = x.size(1), v = w.size(0);
     const float *bias = nullptr;
     bool grads = x.requires_grad();
@@ -347,6 +367,7 @@ PyMethodDef methods[] = {{"describe", describe, METH_O, "pointers, counts and ty
                          {"writable", writable, METH_O, "the first tensor that requires a gradient"},
                          {"written", written, METH_O, "moves the tensors' version counters on"},
                          {"bind", bind, METH_VARARGS, "takes the addresses of the library's functions"},
+                         {"weight", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(weight)), METH_FASTCALL, "whether two tensors are a quantised weight"},
                          {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(sample)), METH_FASTCALL, "the usual call of sample_tokens"},
                          {"logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(logits)), METH_FASTCALL, "the usual call of joiner_logits with a quantised weight"},
                          {"train", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(train)), METH_FASTCALL, "joiner_logits with gradients"},

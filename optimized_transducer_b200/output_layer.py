@@ -59,35 +59,46 @@ def _forward(x, w, pitch, scale, bias, v, out_dtype):
     return out
 
 
+def _check_weight(data, scale, who):
+    """Raises the error for a quantised weight that the kernels cannot read."""
+    for t, name in ((data, "data"), (scale, "scale")):
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{who}: expected {name} to be a tensor, got {type(t).__name__}")
+    if data.dtype != torch.float8_e4m3fn or data.dim() != 2 or data.numel() == 0:
+        raise RuntimeError(f"{who}: data must be a non-empty 2-D float8_e4m3fn tensor")
+    if not data.is_cuda:
+        raise RuntimeError(f"{who}: CUDA tensors only (sm_100a kernels, no CPU path)")
+    if (data.stride(1) != 1 and data.size(1) > 1) or (data.stride(0) % 16 and data.size(0) > 1) \
+            or (data.size(0) > 1 and data.stride(0) < data.size(1)) or data.data_ptr() % 16:
+        raise RuntimeError(f"{who}: data must have a unit column stride, rows a multiple of 16 bytes apart "
+                           f"and a 16-byte aligned base, got strides {tuple(data.stride())}")
+    want = (_blocks(data.size(0)), _blocks(data.size(1)))
+    if scale.dtype != torch.float32 or tuple(scale.shape) != want or not scale.is_contiguous() \
+            or scale.device != data.device:
+        raise RuntimeError(f"{who}: scale must be a contiguous float32 tensor of shape {want} on {data.device}")
+
+
 class Fp8Weight:
     """A quantised projection weight.  ``data``: (V, D) ``torch.float8_e4m3fn``, unit
     column stride, rows a multiple of 16 bytes apart, 16-byte aligned; ``scale``:
     (ceil(V/128), ceil(D/128)) float32, contiguous.  The value of an element is its
-    e4m3 value times its block's scale.  The tensors are used as they are, not copied."""
+    e4m3 value times its block's scale.  The tensors are used as they are, not copied;
+    they may be written to, but a handle keeps the two that it was made with."""
 
-    __slots__ = ("data", "scale")
+    __slots__ = ("_data", "_scale")
 
     def __init__(self, data, scale):
-        who = "Fp8Weight"
-        if (data.dtype is torch.float8_e4m3fn and data.is_cuda and data.is_contiguous() and data.dim() == 2
-                and data.size(1) % 16 == 0 and data.numel() > 0 and data.data_ptr() % 16 == 0
-                and scale.dtype is torch.float32 and scale.is_contiguous() and scale.device == data.device
-                and scale.shape == (_blocks(data.size(0)), _blocks(data.size(1)))):
-            self.data, self.scale = data, scale  # the common case: one pass over the metadata
-            return
-        if data.dtype != torch.float8_e4m3fn or data.dim() != 2 or data.numel() == 0:
-            raise RuntimeError(f"{who}: data must be a non-empty 2-D float8_e4m3fn tensor")
-        if not data.is_cuda:
-            raise RuntimeError(f"{who}: CUDA tensors only (sm_100a kernels, no CPU path)")
-        if (data.stride(1) != 1 and data.size(1) > 1) or (data.stride(0) % 16 and data.size(0) > 1) \
-                or (data.size(0) > 1 and data.stride(0) < data.size(1)) or data.data_ptr() % 16:
-            raise RuntimeError(f"{who}: data must have a unit column stride, rows a multiple of 16 bytes apart "
-                               f"and a 16-byte aligned base, got strides {tuple(data.stride())}")
-        want = (_blocks(data.size(0)), _blocks(data.size(1)))
-        if scale.dtype != torch.float32 or tuple(scale.shape) != want or not scale.is_contiguous() \
-                or scale.device != data.device:
-            raise RuntimeError(f"{who}: scale must be a contiguous float32 tensor of shape {want} on {data.device}")
-        self.data, self.scale = data, scale
+        if not _lib.tensors().weight(data, scale):
+            _check_weight(data, scale, "Fp8Weight")  # says what is wrong
+        self._data, self._scale = data, scale
+
+    @property
+    def data(self):
+        return self._data
+
+    @property
+    def scale(self):
+        return self._scale
 
     @property
     def shape(self):
@@ -174,7 +185,7 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     served = isinstance(weight, Fp8Weight)
     report = 0 if _check_mode() == "off" else _lib.REPORT_ERRORS
     if served:
-        usual = _lib.tensors().logits(joiner_in, weight.data, weight.scale, bias, out_dtype, report)
+        usual = _lib.tensors().logits(joiner_in, weight._data, weight._scale, bias, out_dtype, report)
         if usual is not None:
             return usual
     grads = torch.is_grad_enabled() and (joiner_in.requires_grad or (bias is not None and bias.requires_grad)
@@ -194,7 +205,9 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
 def _check_arguments(joiner_in, weight, bias, out_dtype, served, grads, who):
     """Raises the error for the first argument of :func:`joiner_logits` that will not do."""
     _check_matrix(joiner_in, "joiner_in", who)
-    if not served:
+    if served:
+        _check_weight(weight.data, weight.scale, who)
+    else:
         _check_matrix(weight, "weight", who)
     if weight.device != joiner_in.device or weight.shape[1] != joiner_in.size(1) or weight.shape[0] == 0:
         raise RuntimeError(f"{who}: expected joiner_in (rows, D) and weight (V, D) on one device, got "

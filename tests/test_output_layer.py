@@ -94,3 +94,10 @@ def test_training_calls_argument_errors():
         g, rows, 5, ld, 0, 20, saved, p, 0, p, 0, p, flags, ws, None)
     assert bwd(ws=None) == _lib.ERR_WORKSPACE and bwd(saved=None) == _lib.ERR_WORKSPACE
     assert bwd(g=None) == _lib.ERR_ARGUMENT and bwd(ld=4) == _lib.ERR_ARGUMENT and bwd(flags=_lib.BF16) == _lib.ERR_ARGUMENT
+
+
+def test_a_handle_of_things_that_are_no_tensors_is_refused():
+    q = torch.zeros(3, 16).to(torch.float8_e4m3fn)
+    for data, scale, what in ((None, torch.ones(1, 1), "data"), (q, None, "scale"), (q, [1.0], "scale"), ("w", 3, "data")):
+        with pytest.raises(RuntimeError, match=f"expected {what} to be a tensor"):
+            ot.Fp8Weight(data, scale)

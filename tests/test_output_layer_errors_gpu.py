@@ -17,3 +17,37 @@ def test_a_failed_allocation_is_torchs_own_error():
         with pytest.raises(torch.OutOfMemoryError):
             ot.joiner_logits(x, weight, out_dtype=torch.float32)
     assert float(ot.joiner_logits(x[:4], handle).abs().max()) == 0.0
+
+
+def test_a_handle_keeps_its_tensors():
+    handle = ot.quantize_weight(torch.randn(130, 64, device=DEV))
+    data, scale = handle.data, handle.scale
+    for name, new in (("data", scale), ("scale", None), ("data", 3), ("shape", (1, 1))):
+        with pytest.raises(AttributeError):
+            setattr(handle, name, new)
+    assert handle.data is data and handle.scale is scale
+
+
+def test_a_handle_whose_tensors_changed_since_is_refused():
+    """Checked at every call: tensors can be resized or exchanged behind the handle's back."""
+    x = torch.randn(5, 64, device=DEV)
+
+    def handle():
+        w = torch.randn(130, 64, device=DEV)
+        q = ot.quantize_weight(w)
+        return ot.Fp8Weight(q.data.view(torch.uint8).clone().view(torch.float8_e4m3fn), q.scale.clone())
+
+    for change, what in ((lambda h: h.scale.resize_(1, 1), "scale"), (lambda h: h.data.resize_(130, 48), "expected joiner_in"),
+                         (lambda h: h.data.resize_(0, 64), "data"), (lambda h: h.data.t_(), "data"),
+                         (lambda h: setattr(h.scale, "data", torch.ones(2, 1, device=DEV, dtype=torch.float64)), "scale"),
+                         (lambda h: h.scale.set_(torch.ones(2, 1).to(DEV)[:1]), "scale"),
+                         (lambda h: object.__setattr__(h, "_data", None), "data"), (lambda h: object.__setattr__(h, "_scale", 1.0), "scale")):
+        h = handle()
+        ot.joiner_logits(x, h)
+        change(h)
+        with pytest.raises(RuntimeError, match=what):
+            ot.joiner_logits(x, h)
+    # written to in place: that is what the handle then holds
+    h = handle()
+    h.scale.mul_(2)
+    assert torch.equal(ot.joiner_logits(x, h, out_dtype=torch.float32), 2 * ot.joiner_logits(x, ot.Fp8Weight(h.data, h.scale / 2), out_dtype=torch.float32))
