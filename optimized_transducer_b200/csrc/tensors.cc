@@ -116,6 +116,20 @@ PyObject *writable(PyObject *, PyObject *list) {
   return PyLong_FromSsize_t(found);
 }
 
+// Whether t is a forward-mode dual number (none is while forward mode is switched off).
+bool has_tangent(const at::Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+
+// tangent(list): the index of the first tensor with a forward-mode tangent, -1 when there is none.
+PyObject *tangent(PyObject *, PyObject *list) {
+  PyObject *seq = PySequence_Fast(list, "expected a sequence of tensors");
+  if (seq == nullptr) return nullptr;
+  Py_ssize_t found = -1;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq) && found < 0; ++i)
+    if (THPVariable_Check(PySequence_Fast_GET_ITEM(seq, i)) && has_tangent(THPVariable_Unpack(PySequence_Fast_GET_ITEM(seq, i)))) found = i;
+  Py_DECREF(seq);
+  return PyLong_FromSsize_t(found);
+}
+
 // written(list): the tensors' version counters move on, as after any write that autograd
 // has to know of (inference tensors have none).
 PyObject *written(PyObject *, PyObject *list) {
@@ -316,14 +330,14 @@ PyObject *logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
       Py_RETURN_NONE;
     const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &scale = THPVariable_Unpack(args[2]);
     const at::ScalarType type = reinterpret_cast<THPDtype *>(args[4])->scalar_type;
-    if (!plain_matrix(x) || float_flag(type) < 0 || !plain_weight(w, scale) || w.get_device() != x.get_device() || w.size(1) != x.size(1)) Py_RETURN_NONE;
+    if (!plain_matrix(x) || float_flag(type) < 0 || !plain_weight(w, scale) || has_tangent(x) || has_tangent(scale) || w.get_device() != x.get_device() || w.size(1) != x.size(1)) Py_RETURN_NONE;
     const int64_t rows = x.size(0), d = x.size(1), v = w.size(0);
     const float *bias = nullptr;
     bool grads = x.requires_grad();
     if (args[3] != Py_None) {
       if (!THPVariable_Check(args[3])) Py_RETURN_NONE;
       const at::Tensor &b = THPVariable_Unpack(args[3]);
-      if (!plain_vector(b, at::kFloat, v, x.get_device())) Py_RETURN_NONE;
+      if (!plain_vector(b, at::kFloat, v, x.get_device()) || has_tangent(b)) Py_RETURN_NONE;
       bias = b.data_ptr<float>();
       grads = grads || b.requires_grad();
     }
@@ -365,6 +379,7 @@ PyObject *clip(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {{"describe", describe, METH_O, "pointers, counts and types of a list of tensors"},
                          {"alike", alike, METH_VARARGS, "whether two lists of tensors have the same shapes"},
                          {"writable", writable, METH_O, "the first tensor that requires a gradient"},
+                         {"tangent", tangent, METH_O, "the first tensor with a forward-mode tangent"},
                          {"written", written, METH_O, "moves the tensors' version counters on"},
                          {"bind", bind, METH_VARARGS, "takes the addresses of the library's functions"},
                          {"weight", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(weight)), METH_FASTCALL, "whether two tensors are a quantised weight"},

@@ -179,7 +179,8 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     along the contraction, X in blocks of 128 x 128), ``d bias`` the float32 column
     sums of G.  X and W are kept for the backward pass in e4m3 (one byte per element),
     so overwriting ``joiner_in`` afterwards does no harm.  The gradient is not itself
-    differentiable (``create_graph=True`` is refused).  An :class:`Fp8Weight` has
+    differentiable (``create_graph=True`` is refused), and there is no forward-mode
+    derivative (dual tensors are refused).  An :class:`Fp8Weight` has
     no gradient: ``joiner_in`` may then not require one."""
     who = "joiner_logits"
     served = isinstance(weight, Fp8Weight)
@@ -217,6 +218,11 @@ def _check_arguments(joiner_in, weight, bias, out_dtype, served, grads, who):
         raise RuntimeError(f"{who}: bias must be a contiguous float32 tensor of V entries")
     if out_dtype not in _FLOATS:
         raise RuntimeError(f"{who}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    operands = [joiner_in, weight.scale if served else weight, bias]
+    at = _lib.tensors().tangent(operands)
+    if at >= 0:
+        raise RuntimeError(f"{who}: {('joiner_in', 'weight', 'bias')[at]} carries a forward-mode tangent, and there is no forward-mode "
+                           "derivative: pass its primal (torch.autograd.forward_ad.unpack_dual)")
     if served and grads:
         raise RuntimeError(f"{who}: an Fp8Weight is for inference; pass the weight as a tensor to train")
     if grads and joiner_in.size(0) == 0:

@@ -51,3 +51,24 @@ def test_a_handle_whose_tensors_changed_since_is_refused():
     h = handle()
     h.scale.mul_(2)
     assert torch.equal(ot.joiner_logits(x, h, out_dtype=torch.float32), 2 * ot.joiner_logits(x, ot.Fp8Weight(h.data, h.scale / 2), out_dtype=torch.float32))
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w, b = torch.randn(5, 64, device=DEV), torch.randn(33, 64, device=DEV), torch.randn(33, device=DEV)
+    handle = ot.quantize_weight(w)
+    want = ot.joiner_logits(x, handle, b)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args, what in (((dual(x), w, b), "joiner_in"), ((x, dual(w), b), "weight"), ((x, w, dual(b)), "bias"),
+                           ((dual(x), handle, b), "joiner_in"), ((x, handle, dual(b)), "bias"), ((dual(x), handle), "joiner_in"),
+                           ((dual(x), w.clone().requires_grad_(True), b), "joiner_in"),
+                           ((x, ot.Fp8Weight(handle.data, dual(handle.scale)), b), "weight")):
+            with pytest.raises(RuntimeError, match=f"{what} carries a forward-mode tangent"):
+                ot.joiner_logits(*args)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                ot.joiner_logits(*args)
+        assert torch.equal(ot.joiner_logits(fwd.unpack_dual(dual(x)).primal, handle, b), want)
+    assert torch.equal(ot.joiner_logits(x, handle, b), want)
