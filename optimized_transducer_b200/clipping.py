@@ -30,6 +30,9 @@ def _table(tensors, who, what):
                            f"{tuple(t.shape)}")
     if why == "cpu":
         raise RuntimeError(f"{who}: CUDA tensors only (sm_100a kernels, no CPU path), got one on {t.device}")
+    if why == "dual":
+        raise RuntimeError(f"{who}: one of {what} carries a forward-mode tangent, and there is no forward-mode derivative: pass "
+                           "its primal (torch.autograd.forward_ad.unpack_dual)")
     raise RuntimeError(f"{who}: expected {what} to be on one device, got {t.device} and {tensors[0].device}")
 
 
@@ -61,8 +64,17 @@ def grad_norm(tensors, norm_type=2.0):
     one vector: a 0-dim float32 tensor on their device.  ``tensors``: one dense CUDA
     tensor or an iterable of them, float32, float64, bfloat16 or float16, mixed as one
     likes.  Sums are taken in float64 over groups of at most 32 elements in a fixed
-    order: the same inputs give the same bits."""
-    return _call("grad_norm", _list(tensors), norm_type, False, 0.0, None)
+    order: the same inputs give the same bits.  The norm has no derivative: tensors that
+    require a gradient are refused unless under ``torch.no_grad()``, forward-mode dual
+    tensors always."""
+    who = "grad_norm"
+    tensors = _list(tensors)
+    if torch.is_grad_enabled():
+        at = _lib.tensors().writable(tensors)
+        if at >= 0:
+            raise RuntimeError(f"{who}: tensor {at} requires a gradient, and the norm has no derivative: pass detached tensors "
+                               "or call it under torch.no_grad()")
+    return _call(who, tensors, norm_type, False, 0.0, None)
 
 
 def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):

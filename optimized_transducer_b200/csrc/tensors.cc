@@ -17,6 +17,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <stdexcept>
@@ -49,10 +50,16 @@ template <typename F> PyObject *guarded(F f) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether there may be forward-mode dual numbers at all: asking once spares hundreds of tensors the question (25 ns each).
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+
+// Whether t is a forward-mode dual number (none is while forward mode is switched off).
+bool has_tangent(const at::Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+
 // describe(list) -> (pointers, counts, type flags, device, index, why): three bytes objects
 // with one 64-, 64- and 32-bit entry per tensor, and the CUDA device all are on; or, at the
 // first tensor that will not do, None four times, its index and "tensor" / "layout" /
-// "type" / "cpu" / "device".  "Dense" means one stretch of memory, each element once.
+// "type" / "cpu" / "device" / "dual".  "Dense" means one stretch of memory, each element once.
 PyObject *describe(PyObject *, PyObject *list) {
   PyObject *seq = PySequence_Fast(list, "expected a sequence of tensors");
   if (seq == nullptr) return nullptr;
@@ -62,6 +69,7 @@ PyObject *describe(PyObject *, PyObject *list) {
     std::vector<int64_t> pointers((size_t)n), counts((size_t)n);
     std::vector<int32_t> types((size_t)n);
     int device = -1;
+    const bool duals = forward_mode();
     const char *why = nullptr;
     Py_ssize_t i = 0;
     for (; i < n; ++i) {
@@ -74,6 +82,7 @@ PyObject *describe(PyObject *, PyObject *list) {
       const int flag = type_flag(t.scalar_type());
       if (flag < 0) { why = "type"; break; }
       if (!t.is_contiguous() && !t.is_non_overlapping_and_dense()) { why = "layout"; break; }
+      if (duals && has_tangent(t)) { why = "dual"; break; }
       pointers[(size_t)i] = (int64_t)reinterpret_cast<uintptr_t>(t.numel() > 0 ? t.data_ptr() : nullptr);
       counts[(size_t)i] = t.numel();
       types[(size_t)i] = flag;
@@ -115,9 +124,6 @@ PyObject *writable(PyObject *, PyObject *list) {
   Py_DECREF(seq);
   return PyLong_FromSsize_t(found);
 }
-
-// Whether t is a forward-mode dual number (none is while forward mode is switched off).
-bool has_tangent(const at::Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
 
 // tangent(list): the index of the first tensor with a forward-mode tangent, -1 when there is none.
 PyObject *tangent(PyObject *, PyObject *list) {

@@ -39,7 +39,9 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     stays.  The token is the first index, in index order, at which the kept weights sum
     to more than ``uniforms`` times their total; the log-probability is that of the kept
     weights.  ``temperature=0`` takes the first symbol (log-probability 0).  Each setting
-    is a number or a tensor with one value per row (float32; ``top_k`` int32).
+    is a number or a tensor with one value per row (float32; ``top_k`` int32).  Neither
+    result carries a derivative, of either mode: the log-probabilities of drawn symbols
+    that a loss needs are taken from the logits again.
 
     Tokens are those of 64-bit arithmetic.  ``-inf`` logits are never drawn.  A row
     without a finite maximum (everything ``-inf``, or a NaN or ``+inf`` in it), or whose

@@ -54,3 +54,12 @@ def test_parameters_in_place_of_their_gradients_are_refused():
         ot.clip_grad_norm_([torch.ones(3), p], 1.0)
     with pytest.raises(RuntimeError, match="not the parameters"):
         ot.clip_grad_norm_([torch.ones(3)], 1.0, out=[p])
+
+
+def test_a_norm_that_should_carry_a_gradient_is_refused():
+    p = torch.nn.Parameter(torch.ones(3))
+    for t in (p, 2 * p, torch.autograd.grad((p ** 3).sum(), p, create_graph=True)[0]):
+        with pytest.raises(RuntimeError, match="no derivative"):
+            ot.grad_norm([torch.ones(3), t])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):   # as far as a CPU tensor comes
+            ot.grad_norm([t])
