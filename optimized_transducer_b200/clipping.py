@@ -36,10 +36,15 @@ def _table(tensors, who, what):
     raise RuntimeError(f"{who}: expected {what} to be on one device, got {t.device} and {tensors[0].device}")
 
 
-def _call(who, tensors, norm_type, apply, max_norm, out):
+def _kind(norm_type, who):
     kind = _KINDS.get(float(norm_type))
     if kind is None:
         raise RuntimeError(f"{who}: norm_type must be 1, 2 or inf, got {norm_type}")
+    return kind
+
+
+def _call(who, tensors, norm_type, apply, max_norm, out):
+    kind = _kind(norm_type, who)
     if not tensors:
         raise RuntimeError(f"{who}: no gradients were given")
     grads, counts, types, device = _table(tensors, who, "the gradients")
@@ -88,7 +93,8 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
     Tensors that require a gradient are refused: unlike torch's function this one is not
     given the parameters.  The factor is taken from the norm in float64 (float64 gradients are
     scaled in float64, the others in float32); what is returned is the norm in float32.  The host
-    does not wait for the device.  As in torch an infinite norm scales by 0 and a NaN one by NaN."""
+    does not wait for the device.  As in torch an infinite norm scales by 0 and a NaN one by NaN,
+    and without any tensors (a step in which everything is frozen) the norm is a 0 on the CPU."""
     who = "clip_grad_norm_"
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"{who}: max_norm must not be negative or a NaN, got {max_norm}")
@@ -98,6 +104,9 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, out=None):
     if at >= 0:
         raise RuntimeError(f"{who}: tensor {at} requires a gradient: pass the gradients (p.grad), not the parameters, and no "
                            "gradient that is part of a graph")
+    if not tensors and not written:
+        _kind(norm_type, who)
+        return torch.zeros(())
     norm = _call(who, tensors, norm_type, True, max_norm, None if out is None else written)
     _lib.tensors().written(written)
     return norm

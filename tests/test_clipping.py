@@ -63,3 +63,15 @@ def test_a_norm_that_should_carry_a_gradient_is_refused():
             ot.grad_norm([torch.ones(3), t])
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):   # as far as a CPU tensor comes
             ot.grad_norm([t])
+
+
+def test_nothing_to_clip_is_a_norm_of_zero_as_in_torch():
+    want = torch.nn.utils.clip_grad_norm_([torch.nn.Parameter(torch.ones(3))], 1.0)   # no gradient anywhere
+    for got in (ot.clip_grad_norm_([], 1.0), ot.clip_grad_norm_((t for t in ()), 1.0, norm_type=float("inf")), ot.clip_grad_norm_([], 0.0, out=[])):
+        assert got.shape == want.shape and got.dtype == want.dtype and got.device == want.device and float(got) == float(want) == 0.0
+    with pytest.raises(RuntimeError, match="norm_type"):
+        ot.clip_grad_norm_([], 1.0, norm_type=3.0)
+    with pytest.raises(RuntimeError, match="max_norm"):
+        ot.clip_grad_norm_([], -1.0)
+    with pytest.raises(RuntimeError, match="no gradients|one output per gradient"):
+        ot.clip_grad_norm_([], 1.0, out=[torch.ones(3)])
