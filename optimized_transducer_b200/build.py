@@ -9,6 +9,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -37,6 +38,10 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in deps)
 
 
+def helper_up_to_date():
+    return os.path.isfile(HELPER) and all(os.path.getmtime(d) <= os.path.getmtime(HELPER) for d in (HELPER_SOURCE, HEADERS[-1]))
+
+
 def start_helper():
     """Starts the compilation of ``_tensors.so``."""
     import torch
@@ -45,8 +50,8 @@ def start_helper():
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], cuda)], HELPER_SOURCE, "-o", HELPER,
-           f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+           *[f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], cuda)],
+           HELPER_SOURCE, "-o", HELPER, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
 
@@ -58,15 +63,34 @@ def finish_helper(proc, verbose=False):
         raise RuntimeError(f"g++ failed on {HELPER_SOURCE}")
 
 
+def no_helper(why):
+    warnings.warn(f"_tensors.so was not built ({type(why).__name__}: {why}); it needs g++, torch and the headers of both torch and Python. "
+                  "The loss does without it; joiner_logits, sample_tokens, grad_norm and clip_grad_norm_ do not.", RuntimeWarning, stacklevel=3)
+
+
 def build(force=False, verbose=False):
-    """Compiles every kernel for sm_100a; returns the path of the library."""
-    newest = max(os.path.getmtime(HELPER_SOURCE), os.path.getmtime(HEADERS[-1]))
-    helper = start_helper() if force or not os.path.isfile(HELPER) or os.path.getmtime(HELPER) < newest else None
+    """Compiles every kernel for sm_100a; returns the path of the library.  The library
+    is what has to be there: where the helper cannot be built a warning says so, and
+    what an earlier build left of it is gone."""
+    helper = failed = None
     try:
-        return build_library(force, verbose)
+        if force or not helper_up_to_date():
+            if os.path.isfile(HELPER):
+                os.remove(HELPER)
+            helper = start_helper()
+    except (ImportError, OSError, RuntimeError) as e:
+        failed = e
+    try:
+        lib = build_library(force, verbose)
     finally:
         if helper is not None:
-            finish_helper(helper, verbose)
+            try:
+                finish_helper(helper, verbose)
+            except RuntimeError as e:
+                failed = e
+    if failed is not None:
+        no_helper(failed)
+    return lib
 
 
 def build_library(force=False, verbose=False):
