@@ -189,12 +189,16 @@ def tensors():
     """The compiled helper of the Python layer (``csrc/tensors.cc``), bound to the library."""
     global _helper
     if _helper is None:
-        import torch  # noqa: F401  (its libraries have to be loaded first)
+        from . import build  # imports torch for built_for(): its libraries have to be loaded first
+        here = build.built_for()
         try:
             from . import _tensors as helper
         except ImportError as e:
             raise ImportError("optimized_transducer_b200/_tensors.so is missing or does not load: build it with "
                               f"`python -m optimized_transducer_b200.build` ({e})") from None
+        if getattr(helper, "built_for", None) != here:
+            raise ImportError(f"optimized_transducer_b200/_tensors.so was built for {getattr(helper, 'built_for', 'something older')}, this "
+                              f"is {here}: build it again with `python -m optimized_transducer_b200.build`")
         lib = load()
         helper.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "ot_b200_last_error", "ot_b200_sample", "ot_b200_joiner_logits", "ot_b200_joiner_logits_workspace_bytes",

@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libot_b200.so")
 HELPER = os.path.join(HERE, "_tensors.so")
+HELPER_STAMP = os.path.join(HERE, "_tensors.built")  # what HELPER was built for
 HELPER_SOURCE = os.path.join(CSRC, "tensors.cc")
 SOURCES = ["api.cu", "prep.cu", "logprob.cu", "lattice.cu", "gradient.cu", "noalloc.cu", "pack.cu",
            "exchange.cu", "fused_linear.cu", "fp8.cu", "sample.cu", "clip.cu"]
@@ -38,8 +39,21 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in deps)
 
 
+def built_for():
+    """What the helper is tied to: it uses torch's and Python's C++ and C interfaces."""
+    import torch
+
+    return f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+
+
 def helper_up_to_date():
-    return os.path.isfile(HELPER) and all(os.path.getmtime(d) <= os.path.getmtime(HELPER) for d in (HELPER_SOURCE, HEADERS[-1]))
+    if not (os.path.isfile(HELPER) and os.path.isfile(HELPER_STAMP)):
+        return False
+    t = os.path.getmtime(HELPER)
+    if any(os.path.getmtime(d) > t for d in (HELPER_SOURCE, HEADERS[-1])):
+        return False
+    with open(HELPER_STAMP) as f:
+        return f.read() == built_for()
 
 
 def start_helper():
@@ -50,7 +64,7 @@ def start_helper():
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], cuda)],
+           f'-DOT_BUILT_FOR="{built_for()}"', *[f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], cuda)],
            HELPER_SOURCE, "-o", HELPER, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
@@ -61,6 +75,8 @@ def finish_helper(proc, verbose=False):
         sys.stderr.write(out)
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed on {HELPER_SOURCE}")
+    with open(HELPER_STAMP, "w") as f:
+        f.write(built_for())
 
 
 def no_helper(why):
@@ -75,8 +91,9 @@ def build(force=False, verbose=False):
     helper = failed = None
     try:
         if force or not helper_up_to_date():
-            if os.path.isfile(HELPER):
-                os.remove(HELPER)
+            for old in (HELPER, HELPER_STAMP):
+                if os.path.isfile(old):
+                    os.remove(old)
             helper = start_helper()
     except (ImportError, OSError, RuntimeError) as e:
         failed = e

@@ -398,4 +398,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensors(void) { return PyModule_Create(&module); }
+// built_for: the torch and the Python whose interfaces this file was compiled against.
+PyMODINIT_FUNC PyInit__tensors(void) {
+  PyObject *m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", OT_BUILT_FOR) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
