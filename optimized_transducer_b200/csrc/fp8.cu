@@ -14,8 +14,11 @@
 //
 // Scales.  quantize_kernel takes the smallest power of two s with max|x| / s <= 448 (the
 // largest e4m3 value), 2^-126 at least, 1 for a block of zeros: x / s is then exact but
-// for the rounding to e4m3 itself, and since e4m3 is a floating-point type a scale that is
-// not a power of two would not round less.  A block that holds an infinity or a NaN gets
+// for the rounding to e4m3 itself, which is off by at most max(2^-4 |x|, 2^-10 s): e4m3 is a
+// floating-point type down to 2^-6 and has steps of 2^-9 below, so what is less than 2^-6 s
+// (some 2^-14 of the block's largest) loses bits and what is less than 2^-10 s becomes 0.  A
+// scale that is not a power of two would round the larger ones no less; it could move that
+// border down by up to a factor of two.  A block that holds an infinity or a NaN gets
 // the scale NaN: every product with it is NaN, as it would be without the quantiser.  The
 // product takes any float scales (a checkpoint's).
 #include <cuda_fp8.h>

@@ -108,3 +108,20 @@ def test_gradients(case, types):
     check(gw, value(g.T, 1), value(xv.T, BLOCK))
     # float32 sums over at most 128 rows, joined in a fixed order: (rows + 8) * 2^-24 of the magnitudes
     assert bool(((gb.double() - g.double().sum(0)).abs() <= (rows + 8) * 2.0 ** -24 * g.double().abs().sum(0)).all())
+
+
+@pytest.mark.parametrize("rows_per_block", [1, BLOCK])
+def test_the_stated_bound_of_the_quantiser(rows_per_block):
+    """An element is off by at most max(2^-4 |x|, 2^-10 scale): the second term is that of small
+    ones beside a large one, and it is needed."""
+    from optimized_transducer_b200 import output_layer
+
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    x = torch.randn(300, 500, device=DEV, generator=g) * torch.exp(-15 * torch.rand(300, 500, device=DEV, generator=g))
+    (q, scale), _, _ = output_layer._quantize(x, _lib.FP8_ROWS if rows_per_block == 1 else _lib.FP8_SQUARES)
+    s = scale.t() if rows_per_block == 1 else scale
+    s = s.double().repeat_interleave(rows_per_block, 0)[:300].repeat_interleave(BLOCK, 1)[:, :500]
+    error = (q[:, :500].contiguous().view(torch.float8_e4m3fn).double() * s - x.double()).abs()
+    assert bool((error <= torch.maximum(x.double().abs() / 16, s / 1024)).all())
+    assert bool((error > x.double().abs() / 16).any()) and bool((error == x.double().abs()).any())
