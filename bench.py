@@ -26,8 +26,10 @@ compares that sum with the float64 sum of the ranks' local losses.
 
 ``--impl reference``: the reference's own CPU implementation through its own
 Python layer (``oracle/_ref``: its extension built from its sources plus its
-``transducer_loss.py``; else the C port in ``oracle/``), on the same workload,
-with all host threads.  Under torch.distributed.run only rank 0 works.
+``transducer_loss.py``), on the same workload, with all host threads; where that
+build is not there the line says ``unavailable``.  Under torch.distributed.run
+only rank 0 works.  (``cpu_baseline`` of the default arm falls back to the C port
+in ``oracle/`` and then says so in its ``kind``.)
 
 ``--record-traffic FILE``: not a measurement; reads the csv log of an ncu run of
 this script (metrics dram__bytes_read.sum, dram__bytes_write.sum) and stores the
@@ -304,6 +306,12 @@ def run_reference_arm(args, w):
     if rank != 0:
         return
     from optimized_transducer_b200 import synthetic
+    from oracle import oracle as O
+    if O.load_ref_python() is None:  # a port of it is not the reference
+        print(json.dumps({"impl": "reference",
+                          "unavailable": "oracle/_ref is not built: the reference's sources were not there "
+                                         "(python oracle/build_ref.py)"}), flush=True)
+        return
     n_global, T, U, tg = global_batch(args, w, args.gpus)
     n_sample = reference_sample_size(args, w, T, U, args.ref_utts)
     step, cells, kind, cores, desc = cpu_reference_step_factory(w, T, U, tg, n_sample)
