@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define OT_B200_ABI_VERSION 4
+#define OT_B200_ABI_VERSION 5
 
 typedef enum ot_b200_status {
   OT_B200_OK = 0,
@@ -405,10 +405,21 @@ int ot_b200_joiner_logits(const void *d_x, int64_t rows, int32_t D, int64_t row_
  * each NULL when it is not wanted (need_x, need_w of the forward call must agree with d_gx,
  * d_gw).  q(g), q(g^T) in blocks of 128 along the contraction, w and x in 128 x 128.  The
  * three buffers are 256-byte aligned and as large as ot_b200_joiner_train_bytes says for the
- * same needs; types by flags as above, `flags` may hold OT_B200_REPORT_ERRORS. */
+ * same needs; types by flags as above, `flags` may hold OT_B200_REPORT_ERRORS.  The ..._sized
+ * calls are told how large the buffers are and refuse smaller ones (OT_B200_ERR_WORKSPACE); the
+ * two without sizes, kept for callers that have them, take them to be large enough. */
 int ot_b200_joiner_train_bytes(int64_t rows, int32_t D, int32_t V, int32_t need_x, int32_t need_w,
                                int32_t need_b, uint64_t *saved_out, uint64_t *forward_out,
                                uint64_t *backward_out);
+int ot_b200_joiner_train_forward_sized(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags,
+                                       const void *d_w, int32_t V, int64_t w_stride, uint32_t w_flags,
+                                       const float *d_bias, uint32_t out_flags, int32_t need_x, int32_t need_w,
+                                       void *d_saved, uint64_t saved_bytes, void *d_workspace,
+                                       uint64_t workspace_bytes, void *d_out, void *stream);
+int ot_b200_joiner_train_backward_sized(const void *d_g, int64_t rows, int32_t V, int64_t g_stride, uint32_t g_flags,
+                                        int32_t D, const void *d_saved, uint64_t saved_bytes, void *d_gx,
+                                        uint32_t x_flags, void *d_gw, uint32_t w_flags, float *d_gb, uint32_t flags,
+                                        void *d_workspace, uint64_t workspace_bytes, void *stream);
 int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags,
                                  const void *d_w, int32_t V, int64_t w_stride, uint32_t w_flags,
                                  const float *d_bias, uint32_t out_flags, int32_t need_x, int32_t need_w,

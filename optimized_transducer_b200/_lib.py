@@ -9,7 +9,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libot_b200.so")
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # ot_b200_status
 OK, ERR_ARGUMENT, ERR_CUDA, ERR_WORKSPACE, ERR_INPUT = range(5)
@@ -58,6 +58,8 @@ EXPORTS = (
     "ot_b200_joiner_train_bytes",
     "ot_b200_joiner_train_forward",
     "ot_b200_joiner_train_backward",
+    "ot_b200_joiner_train_forward_sized",
+    "ot_b200_joiner_train_backward_sized",
     "ot_b200_compute_transducer_loss",
     "ot_b200_poll_errors",
     "ot_b200_read_input_status",
@@ -146,6 +148,10 @@ def load():
     lib.ot_b200_joiner_train_forward.argtypes = [vp, i64, i32, i64, u32, vp, i32, i64, u32, vp, u32, i32, i32, vp, vp, vp, vp]
     lib.ot_b200_joiner_train_backward.restype = ctypes.c_int
     lib.ot_b200_joiner_train_backward.argtypes = [vp, i64, i32, i64, u32, i32, vp, vp, u32, vp, u32, vp, u32, vp, vp]
+    lib.ot_b200_joiner_train_forward_sized.restype = ctypes.c_int
+    lib.ot_b200_joiner_train_forward_sized.argtypes = [vp, i64, i32, i64, u32, vp, i32, i64, u32, vp, u32, i32, i32, vp, u64, vp, u64, vp, vp]
+    lib.ot_b200_joiner_train_backward_sized.restype = ctypes.c_int
+    lib.ot_b200_joiner_train_backward_sized.argtypes = [vp, i64, i32, i64, u32, i32, vp, u64, vp, u32, vp, u32, vp, u32, vp, u64, vp]
     lib.ot_b200_scale_gradient.restype = ctypes.c_int
     lib.ot_b200_scale_gradient.argtypes = [vp, i64, vp, u32, vp]
     lib.ot_b200_compute_transducer_loss.restype = ctypes.c_int
@@ -202,7 +208,7 @@ def tensors():
         lib = load()
         helper.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "ot_b200_last_error", "ot_b200_sample", "ot_b200_joiner_logits", "ot_b200_joiner_logits_workspace_bytes",
-            "ot_b200_joiner_train_bytes", "ot_b200_joiner_train_forward", "ot_b200_joiner_train_backward",
+            "ot_b200_joiner_train_bytes", "ot_b200_joiner_train_forward_sized", "ot_b200_joiner_train_backward_sized",
             "ot_b200_clip_workspace_bytes", "ot_b200_clip_gradients")])
         _helper = helper
     return _helper

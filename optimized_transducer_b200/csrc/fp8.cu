@@ -1054,6 +1054,16 @@ int train_layout(int64_t rows, int64_t D, int64_t V, int need_x, int need_w, int
   put(&t->b_product, &t->backward, px > pw ? px : pw);
   return OT_B200_OK;
 }
+
+int check_train_buffers(const char *who, const TrainLayout &t, const void *saved, uint64_t saved_bytes, const void *workspace,
+                        uint64_t workspace_bytes, uint64_t need) {
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || (t.saved && (!saved || reinterpret_cast<uintptr_t>(saved) % 256 != 0)))
+    return fail(OT_B200_ERR_WORKSPACE, "%s: a buffer is missing or not 256-byte aligned", who);
+  if (workspace_bytes < need || saved_bytes < t.saved)
+    return fail(OT_B200_ERR_WORKSPACE, "%s: the workspace has fewer than %llu bytes or the saved buffer fewer than %llu", who,
+                (unsigned long long)need, (unsigned long long)t.saved);
+  return OT_B200_OK;
+}
 }  // namespace
 
 int ot_b200_joiner_train_bytes(int64_t rows, int32_t D, int32_t V, int32_t need_x, int32_t need_w, int32_t need_b,
@@ -1069,15 +1079,15 @@ int ot_b200_joiner_train_bytes(int64_t rows, int32_t D, int32_t V, int32_t need_
   return OT_B200_OK;
 }
 
-int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags, const void *d_w,
-                                 int32_t V, int64_t w_stride, uint32_t w_flags, const float *d_bias, uint32_t out_flags,
-                                 int32_t need_x, int32_t need_w, void *d_saved, void *d_workspace, void *d_out, void *stream) {
+int ot_b200_joiner_train_forward_sized(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags, const void *d_w,
+                                       int32_t V, int64_t w_stride, uint32_t w_flags, const float *d_bias, uint32_t out_flags,
+                                       int32_t need_x, int32_t need_w, void *d_saved, uint64_t saved_bytes, void *d_workspace,
+                                       uint64_t workspace_bytes, void *d_out, void *stream) {
   TrainLayout t;
   int rc = train_layout(rows, D, V, need_x, need_w, 0, &t);
   if (rc) return rc;
-  if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0 ||
-      (t.saved && (!d_saved || reinterpret_cast<uintptr_t>(d_saved) % 256 != 0)))
-    return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_train_forward: a buffer is missing or not 256-byte aligned");
+  rc = check_train_buffers("ot_b200_joiner_train_forward", t, d_saved, saved_bytes, d_workspace, workspace_bytes, t.forward);
+  if (rc) return rc;
   Report report;
   rc = begin_reported_call(out_flags, &report.sticky, &report.seq);
   if (rc) return rc;
@@ -1096,15 +1106,15 @@ int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64
   return rc;
 }
 
-int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int64_t g_stride, uint32_t g_flags, int32_t D,
-                                  const void *d_saved, void *d_gx, uint32_t x_flags, void *d_gw, uint32_t w_flags, float *d_gb,
-                                  uint32_t flags, void *d_workspace, void *stream) {
+int ot_b200_joiner_train_backward_sized(const void *d_g, int64_t rows, int32_t V, int64_t g_stride, uint32_t g_flags, int32_t D,
+                                        const void *d_saved, uint64_t saved_bytes, void *d_gx, uint32_t x_flags, void *d_gw,
+                                        uint32_t w_flags, float *d_gb, uint32_t flags, void *d_workspace, uint64_t workspace_bytes,
+                                        void *stream) {
   TrainLayout t;
   int rc = train_layout(rows, D, V, d_gx != nullptr, d_gw != nullptr, d_gb != nullptr, &t);
   if (rc) return rc;
-  if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0 ||
-      (t.saved && (!d_saved || reinterpret_cast<uintptr_t>(d_saved) % 256 != 0)))
-    return fail(OT_B200_ERR_WORKSPACE, "ot_b200_joiner_train_backward: a buffer is missing or not 256-byte aligned");
+  rc = check_train_buffers("ot_b200_joiner_train_backward", t, d_saved, saved_bytes, d_workspace, workspace_bytes, t.backward);
+  if (rc) return rc;
   if (flags & ~OT_B200_REPORT_ERRORS)
     return fail(OT_B200_ERR_ARGUMENT, "ot_b200_joiner_train_backward: flags may hold OT_B200_REPORT_ERRORS");
   Report report;
@@ -1123,6 +1133,20 @@ int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int6
     rc = matmul(ws + t.gt, row_pitch(rows), at(ws, t.gt_scale), saved + t.xt, row_pitch(rows), at(saved, t.xt_scale), nullptr, V, D, rows,
                 w_flags | flags, ws + t.b_product, t.backward - t.b_product, d_gw, &report, stream);
   return rc;
+}
+
+int ot_b200_joiner_train_forward(const void *d_x, int64_t rows, int32_t D, int64_t x_stride, uint32_t x_flags, const void *d_w,
+                                 int32_t V, int64_t w_stride, uint32_t w_flags, const float *d_bias, uint32_t out_flags,
+                                 int32_t need_x, int32_t need_w, void *d_saved, void *d_workspace, void *d_out, void *stream) {
+  return ot_b200_joiner_train_forward_sized(d_x, rows, D, x_stride, x_flags, d_w, V, w_stride, w_flags, d_bias, out_flags, need_x, need_w,
+                                            d_saved, UINT64_MAX, d_workspace, UINT64_MAX, d_out, stream);
+}
+
+int ot_b200_joiner_train_backward(const void *d_g, int64_t rows, int32_t V, int64_t g_stride, uint32_t g_flags, int32_t D,
+                                  const void *d_saved, void *d_gx, uint32_t x_flags, void *d_gw, uint32_t w_flags, float *d_gb,
+                                  uint32_t flags, void *d_workspace, void *stream) {
+  return ot_b200_joiner_train_backward_sized(d_g, rows, V, g_stride, g_flags, D, d_saved, UINT64_MAX, d_gx, x_flags, d_gw, w_flags, d_gb,
+                                             flags, d_workspace, UINT64_MAX, stream);
 }
 
 }  // extern "C"

@@ -160,8 +160,8 @@ decltype(&ot_b200_sample) f_sample;
 decltype(&ot_b200_joiner_logits) f_logits;
 decltype(&ot_b200_joiner_logits_workspace_bytes) f_logits_bytes;
 decltype(&ot_b200_joiner_train_bytes) f_train_bytes;
-decltype(&ot_b200_joiner_train_forward) f_train_forward;
-decltype(&ot_b200_joiner_train_backward) f_train_backward;
+decltype(&ot_b200_joiner_train_forward_sized) f_train_forward;
+decltype(&ot_b200_joiner_train_backward_sized) f_train_backward;
 decltype(&ot_b200_clip_workspace_bytes) f_clip_bytes;
 decltype(&ot_b200_clip_gradients) f_clip;
 
@@ -285,7 +285,8 @@ struct JoinerLogits : torch::autograd::Function<JoinerLogits> {
     at::Tensor out = at::empty({rows, v}, x.options().dtype(type).requires_grad(false));
     check(f_train_forward(x.data_ptr(), rows, (int32_t)d, rows > 1 ? x.stride(0) : d, (uint32_t)float_flag(x.scalar_type()), w.data_ptr(),
                           (int32_t)v, v > 1 ? w.stride(0) : d, (uint32_t)float_flag(w.scalar_type()), bias ? bias->data_ptr<float>() : nullptr,
-                          (uint32_t)(float_flag(type) | report), need_x, need_w, saved.data_ptr(), ws.data_ptr(), out.data_ptr(), stream_of(x)));
+                          (uint32_t)(float_flag(type) | report), need_x, need_w, saved.data_ptr(), size[0], ws.data_ptr(), size[1],
+                          out.data_ptr(), stream_of(x)));
     ctx->save_for_backward({saved});
     ctx->saved_data["meta"] = std::vector<int64_t>{rows, d, v, (int64_t)x.scalar_type(), (int64_t)w.scalar_type(), need_x, need_w, need_b,
                                                    (int64_t)size[2], report};
@@ -307,9 +308,9 @@ struct JoinerLogits : torch::autograd::Function<JoinerLogits> {
     if (m[6]) gw = at::empty({v, d}, options.dtype(w_type));
     if (m[7]) gb = at::empty({v}, options.dtype(at::kFloat));
     check(f_train_backward(g.data_ptr(), rows, (int32_t)v, rows > 1 ? g.stride(0) : v, (uint32_t)float_flag(g.scalar_type()), (int32_t)d,
-                           saved.data_ptr(), gx.defined() ? gx.data_ptr() : nullptr, (uint32_t)float_flag(x_type),
+                           saved.data_ptr(), (uint64_t)saved.numel(), gx.defined() ? gx.data_ptr() : nullptr, (uint32_t)float_flag(x_type),
                            gw.defined() ? gw.data_ptr() : nullptr, (uint32_t)float_flag(w_type), gb.defined() ? gb.data_ptr<float>() : nullptr,
-                           (uint32_t)m[9], ws.data_ptr(), stream_of(g)));
+                           (uint32_t)m[9], ws.data_ptr(), (uint64_t)m[8], stream_of(g)));
     return {gx, gw, gb, none, none};
   }
 };

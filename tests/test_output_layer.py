@@ -101,3 +101,20 @@ def test_a_handle_of_things_that_are_no_tensors_is_refused():
     for data, scale, what in ((None, torch.ones(1, 1), "data"), (q, None, "scale"), (q, [1.0], "scale"), ("w", 3, "data")):
         with pytest.raises(RuntimeError, match=f"expected {what} to be a tensor"):
             ot.Fp8Weight(data, scale)
+
+
+def test_training_calls_refuse_small_buffers():
+    lib = _lib.load()
+    keep, p = _memory()
+    n = [ctypes.c_uint64() for _ in range(3)]
+    assert lib.ot_b200_joiner_train_bytes(4, 20, 5, 1, 1, 1, *[ctypes.byref(x) for x in n]) == _lib.OK
+    saved, forward, backward = (x.value for x in n)
+    fwd = lambda s=saved, w=forward: lib.ot_b200_joiner_train_forward_sized(  # noqa: E731
+        p, 4, 20, 20, 0, p, 5, 20, 0, None, _lib.FP64, 1, 1, p, s, p, w, p, None)
+    bwd = lambda s=saved, w=backward: lib.ot_b200_joiner_train_backward_sized(  # noqa: E731
+        p, 4, 5, 5, 0, 20, p, s, p, 0, p, 0, p, _lib.FP64, p, w, None)
+    for call, need in ((fwd, forward), (bwd, backward)):
+        for kw in (dict(s=saved - 1), dict(w=need - 1), dict(s=0), dict(w=0)):
+            assert call(**kw) == _lib.ERR_WORKSPACE, kw
+            assert "fewer than" in _lib.last_error()
+    assert bwd() == _lib.ERR_ARGUMENT                 # past the sizes: the flag that it does not know
