@@ -55,6 +55,8 @@ struct SampleArgs {
   float *logprob;
 };
 
+constexpr float kLeastNormal = 1.17549435e-38f;  // 2^-126
+
 __device__ __forceinline__ float inf_f() { return __int_as_float(0x7f800000); }
 
 __device__ __forceinline__ float warp_max_f(float v) {
@@ -434,6 +436,10 @@ sample_kernel(const SampleArgs a) {
   float w[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) w[e] = weight(x[e]);
+  if (temperature < kLeastNormal) {  // 1 / temperature is no float: such a row's weights come from double
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = (float)exact(x[e]);
+  }
   // The sum of f over the thread's elements: in wide rows fours in float, those in double
   using S = typename TeamT::Sum;
   const auto sum_of = [&](auto f) {
@@ -636,7 +642,7 @@ sample_kernel(const SampleArgs a) {
       const S wb = (S)weight(hi), n = ceil((goal - above) / wb);
       ties = (int)fmin(fmax(n, S(1)), (S)equal);
       const S at = above + (S)ties * wb - goal;
-      if (!(wb > S(0)) || fabs(at) <= near || (ties > 1 && fabs(at - wb) <= near)) {
+      if (temperature < kLeastNormal || !(wb > S(0)) || fabs(at) <= near || (ties > 1 && fabs(at - wb) <= near)) {
         double above64;
         const double goal64 = (double)top_p * exact_sums(hi, above64), wb64 = exact(hi);
         double m = ceil((goal64 - above64) / wb64);

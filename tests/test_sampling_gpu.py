@@ -247,3 +247,18 @@ def test_many_rows_on_another_stream_and_in_a_captured_graph():
     u.copy_(1 - u)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+@pytest.mark.parametrize("v", [40, 700, 3000, 20000])
+def test_subnormal_temperatures(v):
+    """Logits a few of the smallest floats apart and a temperature of that size: the exponents
+    are ordinary numbers although 1 / temperature is none in float32."""
+    rng = np.random.default_rng(v + 3)
+    least = 2.0 ** -149
+    x = torch.from_numpy(-least * rng.integers(0, 40, (12, v))).float()
+    u = torch.from_numpy(rng.random(12)).float()
+    for t in (least, 3 * least, 20 * least, 1000 * least, 2.0 ** -127, 2.0 ** -126):
+        for f in (dict(), dict(p=0.6), dict(p=0.95, k=30), dict(m=0.05), dict(k=9, p=0.9, m=1e-3)):
+            check(x, u, t=t, **f)
+    t = torch.from_numpy(rng.choice([0.0, least, 5 * least, 1e-40, 1e-38, 1.0], 12)).float()
+    check(x, u, t=t, p=0.8)
