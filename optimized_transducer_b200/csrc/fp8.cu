@@ -445,7 +445,7 @@ template <int kTileN> struct MatmulShared {
 //   warp 0   TMA producer: a (128 x 128) and b (kTileN x 128) boxes into the ring
 //   warp 1   MMA issuer
 //   warps 4..  epilogue: warp % 4 picks the TMEM lanes (rows), the rest the columns
-// Measured (116 250 rows): logits from D = 512 to V = 5000 470-510 us, dX (V -> D) 350 us =
+// Measured (116 250 rows): logits from D = 512 to V = 5000 470-530 us, dX (V -> D) 350 us =
 // 1.7 PFLOP/s, dW 373 us.  A K block takes about 1 150 cycles, of which the epilogue is busy for
 // 990, and the SMs' clock falls to 1.5 - 1.7 GHz under this load; sixteen epilogue warps of 64
 // columns, a leaner wait and other depths of the reads all came out within 3 % of this form.

@@ -345,7 +345,8 @@ __device__ __noinline__ double exact_weight_call(float x, float top, double inve
 // 53 us without a filter, 157 us with top-p (about 1 900 instructions per row; the issue slots
 // are 85 % used), 24 us would be the read.  A few rows are bound by the chain of a search's
 // steps (a comparison per logit, then a reduction: 350 cycles in a warp, 600 in a block, 1.5 us
-// in a cluster): 256 x 5000 with all filters 26 us, 16 x 100003 with top-p and min-p 52 us.
+// in a cluster): 256 x 5000 with all filters 25 us, 16 x 100003 with top-p and min-p 49 - 72 us
+// (over a dozen sets of inputs: by how often the slowest row asks for its sums in double).
 // Tried and slower: four or eight pivots per step (the instructions grow faster than the
 // steps fall: 256 x 5000 46 us with eight), pivots by the secant of the logarithm of what lies
 // below (one end of the bracket stays put), a bisection that keeps both ends on logits from
@@ -725,7 +726,19 @@ cudaError_t launch(SampleArgs a, cudaStream_t s) {
 }
 
 // A row that fits the registers of a warp stays with one warp; wider ones take a block, and
-// the widest a cluster of eight, whose blocks hold a piece of the row each.
+// the widest a cluster of eight, whose blocks hold a piece of the row each.  The rule: the
+// narrowest form that holds the row.  At every width and number of rows measured it is the
+// fastest, because a step's instructions grow with the logits per thread and its barrier with
+// the warps; a form more than the row needs costs (us, float, top-p 0.9, the row's own form and
+// the next wider one; a few rows without a filter take 5 in both):
+//     V = 128     40 000 rows    44   69      V = 6144     4096 rows   186   351
+//     V = 512     40 000 rows    80  134      V = 8192     4096 rows   359   470
+//     V = 1024    40 000 rows   146 1266      V = 16384     256 rows    50   456
+//     V = 4096      4096 rows   154  178      V = 64000     256 rows   519   629
+//     V = 5000 (the 6144 form)  4096 rows 182 345, 16 rows 12.4 14.5
+//     V = 130000    256 rows    702 1397
+// So 16 385 columns cost nine times what 16 384 do: a cluster of eight for a row that three
+// blocks would hold.
 template <typename T> cudaError_t launch_by_width(const SampleArgs &a, cudaStream_t s) {
   if (a.V <= 128) return launch<T, 1, 1, 1, 4>(a, s);
   if (a.V <= 512) return launch<T, 1, 1, 4, 4>(a, s);

@@ -173,7 +173,9 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     quantised in blocks of 1 x 128 and a weight tensor in blocks of 128 x 128; with
     ``s`` the block's scale (between 1/448 and 1/224 of its largest magnitude) an element
     is off by at most ``max(2^-4 |x|, 2^-10 s)``, so one below ``2^-10 s`` becomes 0.  The
-    sums are float32, rounded once to ``out_dtype``.  A block that holds an infinity or a NaN makes its products NaN.
+    sums are float32, rounded once to ``out_dtype``.  The scales of two blocks that meet are
+    multiplied in float32 first: magnitudes that multiply to 2^144 and more overflow there
+    even if the largest ones never meet, below 2^-132 the pair's share is lost.  A block that holds an infinity or a NaN makes its products NaN.
 
     With a weight tensor the call is differentiable: ``d joiner_in = q(G) q(W)`` and
     ``d weight = q(G^T) q(X)`` in e4m3 (the gradient G of the logits in blocks of 128
