@@ -183,7 +183,8 @@ def joiner_logits(joiner_in, weight, bias=None, out_dtype=torch.bfloat16):
     sums of G.  X and W are kept for the backward pass in e4m3 (one byte per element),
     so overwriting ``joiner_in`` afterwards does no harm.  The gradient is not itself
     differentiable (``create_graph=True`` is refused), and there is no forward-mode
-    derivative (dual tensors are refused).  An :class:`Fp8Weight` has
+    derivative (dual tensors are refused); a call whose gradients are wanted needs at least
+    one row.  An :class:`Fp8Weight` has
     no gradient: ``joiner_in`` may then not require one."""
     who = "joiner_logits"
     served = isinstance(weight, Fp8Weight)
